@@ -37,6 +37,10 @@ extern "C" {
 #define PKV_ERR_UNSUPPORTED 801
 #define PKV_ERR_NO_BLOCKS 802  /* the pool cannot satisfy a request */
 
+/* Element types of rows (dtype arguments). */
+#define PKV_BF16 0
+#define PKV_FP16 1
+
 const char* pkv_strerror(int status);
 /* ABI version: bumps when a signature changes. */
 int pkv_version(void);
@@ -336,6 +340,125 @@ int pkv_attn_prefill_e4m3_split(const void* q, const void* kcache, const void* v
                                 const int32_t* cu, int seqs, const int32_t* block_table, int max_blocks,
                                 int block_size, void* out, float scale, const int32_t* outs, int spec, int T,
                                 int64_t num_blocks, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Device: a step planned on the GPU (block tables, slot map, row metadata)
+ * ------------------------------------------------------------------------- */
+
+/* What pkv_kv_reserve, pkv_kv_fill and pkv_kv_pad do on the host, from request
+ * lengths that lie on the GPU: for decode loops that run several steps, or
+ * replay a graph, without the host (the reference's scheduler plans every step
+ * on the host, src/sched.rs:895-1187). All arrays are device int32.
+ *
+ * Row s < nrows holds len[s] positions in held[s] pages (block_table row s,
+ * [nrows][max_blocks]) and feeds ntok[s] more tokens (0: none). A row that
+ * needs pages takes the last ones of free_list[0 .. *free_count) in list order,
+ * rows in order (pkv_pool_take), and they are written behind its held pages:
+ * need = max(0, ceil((len + ntok) / block_size) - held). Without a free list
+ * (both pointers null) the tables are taken as they are. ntok[s] < 0 makes a
+ * padding row of -ntok[s] tokens (pkv_kv_pad). The step's tokens are the rows'
+ * tokens one after the other: cu[0 .. nrows]; token k of a row has pos =
+ * len + k, tok_seq = s and slot_map = the slot of pos (-1 where the page id is
+ * outside [0, num_blocks)); tokens of padding rows and of rows with a status
+ * have pos = k and slot -1, tokens past the last row up to T have pos 0, slot
+ * -1 and tok_seq 0, so that a step captured for T tokens never stores them.
+ * limits[s] = pages * block_size - 1 (-1 for padding rows and rows with a
+ * status). len_out, held_out, free_count_out (may be null): the state after
+ * the step; each may be its input. status[s]: 0; PKV_ERR_NO_BLOCKS where the
+ * free pages do not cover the row and the rows before it that need pages (it
+ * takes none, nor do later rows that need some); PKV_ERR_INVALID where its
+ * lengths do not fit its table (or, without a free list, its pages), or its
+ * tokens do not fit T (no tokens then, nor any later row's). Rows with a
+ * status keep their state.
+ * PKV_ERR_UNSUPPORTED: num_blocks * block_size or max_blocks * block_size
+ * above 2^31 - 1, num_blocks or T of 2^29 or more. */
+int pkv_plan_step(const int32_t* len, const int32_t* held, const int32_t* ntok, int nrows, int32_t* block_table,
+                  int max_blocks, int block_size, int64_t num_blocks, const int32_t* free_list,
+                  const int32_t* free_count, int T, int32_t* pos, int32_t* slot_map, int32_t* tok_seq, int32_t* cu,
+                  int32_t* limits, int32_t* len_out, int32_t* held_out, int32_t* free_count_out, int32_t* status,
+                  void* stream);
+
+/* Gives pages back: row s with 0 <= new_len[s] <= len[s] keeps new_len[s]
+ * positions and ceil(new_len / block_size) pages; the pages past them go to
+ * the end of free_list, rows in order, pages in table order, and *free_count
+ * grows (pkv_kv_truncate with free_pages; 0: pkv_kv_release). Other rows
+ * (new_len[s] < 0: leave) stay as they are. free_list holds num_blocks ids;
+ * pages belong to one row each (shared pages are the host manager's). */
+int pkv_plan_truncate(const int32_t* new_len, int32_t* len, int32_t* held, int nrows, const int32_t* block_table,
+                      int max_blocks, int block_size, int64_t num_blocks, int32_t* free_list, int32_t* free_count,
+                      void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Device: rotary positions on three axes, and rows rotated by them
+ * ------------------------------------------------------------------------- */
+
+/* The `rope` argument of pkv_attn_prep, pkv_rope_rows and pkv_mtp_next for
+ * sequences with images and videos. A request's media are spans, spans[i] =
+ * {start, t, h, w, step} (int32): the t h w tokens from index start of the
+ * sequence on, laid out [t][h][w] (after any merging of patches), sorted by
+ * start, not overlapping; request r has spans span_cu[r] .. span_cu[r+1]-1.
+ * Text takes the next position on all three axes. A span that starts at
+ * position b gives token (i, j, k) the position (time b + i step, height
+ * b + j, width b + k); the token behind it has b + max((t - 1) step + 1, h, w).
+ * pkv_rope_spans writes base[i] = b of every span, once per request (its
+ * prefix sum over the request's spans). A span with a size below 1, a step
+ * below 0 or more than 2^31 - 1 tokens is text. */
+int pkv_rope_spans(const int32_t* span_cu, const int32_t* spans, int n_req, int n_spans, int32_t* base, void* stream);
+
+/* The positions of a step's rows (also of generated tokens, behind every
+ * span): row t is token pos[t] of request tok_seq[t] (pkv_plan_step's and
+ * pkv_kv_fill's arrays); rope[axis * rope_stride + t] for axis 0 (time), 1
+ * (height), 2 (width). Rows of a request outside [0, n_req) have pos[t] on all
+ * axes. rope_stride >= T. */
+int pkv_rope_positions(const int32_t* pos, const int32_t* tok_seq, int T, const int32_t* span_cu, const int32_t* spans,
+                       const int32_t* base, int n_req, int n_spans, int32_t* rope, int rope_stride, void* stream);
+
+/* Norm (optional) and rotation of a step's q and k rows, for heads of D = 64,
+ * 128 or 256 dims and rows that go to pkv_attn_packed or to a cache by
+ * pkv_append (pkv_attn_prep does both at once for this cache's 256 dims):
+ *   y = x * w / sqrt(mean(x^2) + eps)        (w = q_norm / k_norm [D] f32; null: y = x)
+ *   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin), angle = rope[axes[i]] * inv_freq[i]
+ * for pair i < rot / 2 of the first rot dims, (a, b) = (i, i + rot / 2), or
+ * (2 i, 2 i + 1) with adjacent; dims from rot on are y. axes[i] (int32) is the
+ * axis of pair i (values other than 1 and 2: time), so any sections of axes,
+ * one after the other or interleaved. Angles are exact to 2^-40 of a turn at
+ * any position, the arithmetic is f32, rounded once at the end (pkv_attn_prep
+ * rounds where the reference does). Rows and strides as pkv_attn_packed; out
+ * may be in (same strides), else they may not overlap. rot is a multiple of 16
+ * (0: norm alone). Hq or Hkv may be 0. */
+int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                  void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row,
+                  int64_t k_out_head, int Hq, int Hkv, int D, int dtype, const float* q_norm, const float* k_norm,
+                  float eps, const int32_t* rope, int rope_stride, const int32_t* axes, const float* inv_freq, int rot,
+                  int adjacent, int T, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Device: attention over whole prompts that are kept in no cache
+ * ------------------------------------------------------------------------- */
+
+/* Causal attention over a batch of packed prompts: sequence s < seqs holds
+ * rows cu[s] .. cu[s+1]-1 (cu: device, seqs + 1 offsets that do not decrease,
+ * within [0, T]); every row attends the rows of its sequence up to itself:
+ * out[t][h] = softmax_j(scale q[t][h] . k[j][h / G]) . v[j][h / G], times
+ * sigmoid(gate[t][h]) where gate is not null, G = Hq / Hkv any whole number.
+ * For prompts that nothing decodes after (embedding, scoring, rerank): no
+ * pages, no slots, any head count; pkv_attn_prefill is the paged form.
+ * Rows of D = 64, 128 or 256 contiguous elements of dtype (PKV_BF16,
+ * PKV_FP16); *_row and *_head are the strides in elements between rows
+ * (tokens) and between heads, multiples of 8, 0 .. 2^24 (the views of a
+ * projection row [Hq x (q | gate) | k | v] as they are; out rows may not
+ * overlap, nor overlap inputs). Pointers 16-byte aligned. Scores, sums and
+ * values in f32; weights are rounded to dtype for the second product and the
+ * output once, after the gate. Rows outside every sequence are left as they
+ * are; an empty sequence is skipped; offsets outside [0, T] are clamped. An
+ * infinite or NaN value, key or query reaches exactly the rows that attend
+ * it. scale is finite and above 0. PKV_ERR_UNSUPPORTED for other types, dims
+ * or groups, or T G above 2^30. No workspace. No reference counterpart (the
+ * reference attends through its pages only, src/model.rs:2438-2493). */
+int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                    const void* v, int64_t v_row, int64_t v_head, const void* gate, int64_t gate_row,
+                    int64_t gate_head, void* out, int64_t out_row, int64_t out_head, const int32_t* cu, int seqs, int T,
+                    int Hq, int Hkv, int D, int dtype, float scale, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Device: attention input preparation (the reference's append site)

@@ -25,7 +25,7 @@ COMMON = [
 # kernel of the library changes). 24 x 4 draft rows at 12 / 2 heads, 900 to
 # 16,000 keys, 115.0 -> 106.1 us; 4 x 4 over 500 keys 17.1 -> 16.1.
 FLAGS = COMMON + ["-fPIC", "-shared", "-mllvm", "-amdgpu-mfma-vgpr-form"]
-SOURCES = ["pkv_capi.hip", "pkv_host.cpp"]
+SOURCES = ["pkv_capi.hip", "pkv_packed_capi.hip", "pkv_steps_capi.hip", "pkv_host.cpp"]
 
 
 def _run(cmd, what, verbose):

@@ -7,7 +7,7 @@
 #include "pkv_prefill.hip"
 #include "pkv_verify.hip"
 #include "pkv_prep.hip"
-#include "../../include/pkv.h"
+#include "pkv_entry.h"
 
 #include <hip/hip_ext.h>
 
@@ -24,13 +24,6 @@ template <class K>
 K by_group(int G, K g1, K g2, K g4, K g6, K g8) {
     return G == 1 ? g1 : G == 2 ? g2 : G == 4 ? g4 : G == 6 ? g6 : g8;
 }
-
-
-int status_of(hipError_t e) { return e == hipSuccess ? PKV_OK : (int)e; }
-
-int launch_status() { return status_of(hipGetLastError()); }
-
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 int vec_mode(const void* a, const void* b, const void* c, const void* d, int64_t stride, int row_bytes) {
     if (row_bytes % 16 == 0 && stride % 16 == 0 && aligned(a, 16) && aligned(b, 16) && aligned(c, 16) &&

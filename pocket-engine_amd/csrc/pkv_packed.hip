@@ -1,0 +1,453 @@
+// Attention over whole prompts that are kept in no cache (pkv_attn_packed):
+// packed rows of sequences of different lengths, causal, grouped heads, bf16
+// or fp16, heads of 64, 128 or 256 dims.
+//
+// For query i of a sequence and head h, with kv head h / G:
+//   x_j = scale q_i . k_j,  j = 0 .. i
+//   out = sum_j e^(x_j - m) v_j / sum_j e^(x_j - m),  m = max_j x_j,
+// times sigmoid(gate) where gate rows are given. One pass over the keys with
+// the running maximum (kept in log2 units), sum and weighted values.
+//
+// A workgroup takes RW consecutive rows of one sequence and one kv head, a row
+// being a (query, head of the group) pair, row = query * G + head: every G
+// shares a K / V tile among its heads, short prompts fill tiles, and a wave's
+// 32 rows span only 32 / G queries, so little of a diagonal tile is masked
+// work. Scores are computed transposed, S^T[key][row] = K Q^T: a lane then
+// holds one row's 16 scores of a 32-key block (keys 8 (r / 4) + 4 (lane / 32)
+// + r % 4), the softmax needs one exchange between the lane's halves, and the
+// weights are the B operand of O^T[dim][row] += V^T P^T as they stand; V^T
+// fragments are read from the row-major V tile by ds_read_b64_tr_b16.
+#pragma once
+#include "pkv_rows.h"
+
+namespace pkv {
+
+struct PackedParams {
+    const uint16_t *q, *k, *v, *gate;  // gate: null for none
+    uint16_t* out;
+    // row (token) and head strides in elements
+    long q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, o_row, o_head;
+    const int* cu;
+    int seqs, T, Hkv, G;
+    float scale2;  // scale * log2(e)
+};
+
+// Shapes of a workgroup: D dims a head, NW waves of 32 NQB rows, tiles of KB
+// blocks of 32 keys, two stages.
+template <int D, int NQB, int KB, int NW>
+struct PackedTile {
+    static constexpr int RW = 32 * NQB * NW, BK = 32 * KB, THREADS = 64 * NW;
+    // A 32-row block of K or V in LDS: NG groups of 1,024 bytes, one LDS DMA
+    // instruction each; row r lies in group r % NG at (r / NG) 2 D bytes.
+    // K groups are 1,056 bytes apart (1,040 at 256 dims) and rows with bit 3
+    // set have their 16-byte pieces swapped in pairs, so the 16 rows that a
+    // quarter-wave reads with ds_read_b128 start at distinct 16-byte places
+    // modulo 256; V groups are 1,088 bytes apart, so the 4 rows x 64 bytes of
+    // a half-wave's transposing read lie on distinct banks.
+    static constexpr int NG = D / 16;
+    static constexpr int KG = D == 256 ? 1040 : 1056, VG = 1088;
+    static constexpr int KBLK = NG * KG, VBLK = NG * VG;
+    static constexpr int STAGE = KB * (KBLK + VBLK);
+    static constexpr int PER = KB * NG / NW;  // groups of K (and of V) that a wave requests per tile
+    static constexpr int RR = 68;             // staged output row, floats of 64 dims
+    static constexpr int EPI = NW * 32 * RR * 4;
+    static constexpr int LDS = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+    static_assert(KB * NG % NW == 0 && NG % PER == 0, "a wave's groups lie in one block");
+    static __device__ __forceinline__ constexpr int swap(int r) { return D == 256 ? 0 : (r >> 3) & 1; }
+};
+
+// Sequence s and its tile x of this workgroup among the batch's tiles, numbered
+// from the last: later tiles of a sequence attend more keys, so the longest
+// work is started first. Each thread counts the tiles of `per` sequences, the
+// prefix sums over threads find the one that holds the tile. False where the
+// grid has more workgroups than the batch has tiles.
+template <int RW, int NW>
+__device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile, int& c0, int& n, int& x) {
+    __shared__ int wsum[NW], found[3];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (p.seqs + 64 * NW - 1) / (64 * NW);
+    const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
+    // offsets outside [0, T] are clamped: no row out of range is touched
+    auto at = [&](int s) { return max(0, min(p.cu[s], p.T)); };
+    auto tiles = [&](int a, int b) { return b > a ? ((b - a) * p.G + RW - 1) / RW : 0; };
+    int sum = 0, a = s0 < s1 ? at(s0) : 0;
+    for (int s = s0; s < s1; s++) {
+        const int b = at(s + 1);
+        sum += tiles(a, b);
+        a = b;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        if (w < wave) before += wsum[w];
+        total += wsum[w];
+    }
+    if (tile >= total) return false;
+    const int want = total - 1 - tile;
+    before += incl - sum;
+    if (before <= want && want < before + sum) {
+        int a = at(s0);
+        for (int s = s0; s < s1; s++) {
+            const int b = at(s + 1), k = tiles(a, b);
+            if (want < before + k) {
+                found[0] = a;
+                found[1] = b - a;
+                found[2] = want - before;
+                break;
+            }
+            before += k;
+            a = b;
+        }
+    }
+    __syncthreads();
+    c0 = __builtin_amdgcn_readfirstlane(found[0]);
+    n = __builtin_amdgcn_readfirstlane(found[1]);
+    x = __builtin_amdgcn_readfirstlane(found[2]);
+    return true;
+}
+
+template <class E, int D, int NQB, int KB, int NW>
+__device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, int c0, int n, int x, int kvh) {
+    using S = PackedTile<D, NQB, KB, NW>;
+    constexpr int NG = S::NG, BK = S::BK;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lq = lane & 31,
+              lh = lane >> 5;
+    const int rows = n * p.G;                 // of the sequence
+    const int row0 = x * S::RW;               // first of this tile
+    const int wrow = row0 + 32 * NQB * wave;  // first of this wave
+    // Query and head in the group of row r; rows past the sequence stand for
+    // its last one and are not written.
+    auto split = [&](int r, int& qi, int& hh) {
+        r = min(r, rows - 1);
+        qi = r / p.G;
+        hh = r - qi * p.G;
+    };
+    const int L = (min(row0 + S::RW, rows) - 1) / p.G + 1;  // keys of this tile
+    const int ntiles = (L + BK - 1) / BK;
+    // the wave's last query (below the first key: no rows)
+    const int last = wrow < rows ? (min(wrow + 32 * NQB, rows) - 1) / p.G : -1;
+
+    // Requests of K and V rows, straight to LDS: the wave's PER groups from
+    // group g0 of block j0 on, lane i bringing 16 bytes of row g + NG (i /
+    // (D / 8)) (K: of the piece that belongs at its place).
+    constexpr int CH = D / 8;  // 16-byte pieces per row
+    const int j0 = wave * S::PER / NG, g0 = wave * S::PER % NG;
+    const int lb = lane / CH, lc = lane % CH;
+    const uint32_t k_row2 = (uint32_t)p.k_row * 2, v_row2 = (uint32_t)p.v_row * 2;
+    const uint32_t piece_k = 16 * (lc ^ (D == 128 ? lb & 1 : D == 64 ? (lb >> 1) & 1 : 0)), piece_v = 16 * lc;
+    const uint32_t off_k = (uint32_t)(NG * lb) * k_row2 + piece_k, off_v = (uint32_t)(NG * lb) * v_row2 + piece_v;
+    const char* kb = reinterpret_cast<const char*>(p.k + c0 * p.k_row + kvh * p.k_head);
+    const char* vb = reinterpret_cast<const char*>(p.v + c0 * p.v_row + kvh * p.v_head);
+    const uint32_t lds0 = lds_addr(smem);
+    auto request = [&](int k0, int buf) __attribute__((always_inline)) {
+        const uint32_t lk = lds0 + buf * S::STAGE + j0 * S::KBLK + g0 * S::KG;
+        const uint32_t lv = lds0 + buf * S::STAGE + KB * S::KBLK + j0 * S::VBLK + g0 * S::VG;
+        const int r0 = k0 + 32 * j0 + g0;
+        if (k0 + BK <= L) {
+            const char* kg = kb + (size_t)r0 * k_row2;
+            const char* vg = vb + (size_t)r0 * v_row2;
+#pragma unroll
+            for (int i = 0; i < S::PER; i++) dma16_s(kg + (size_t)i * k_row2, off_k, lk + i * S::KG);
+#pragma unroll
+            for (int i = 0; i < S::PER; i++) dma16_s(vg + (size_t)i * v_row2, off_v, lv + i * S::VG);
+        } else {
+            // the last tile: rows past the keys stand for the last key
+#pragma unroll
+            for (int i = 0; i < S::PER; i++) {
+                const int u = min(r0 + i, L - 1), l = min(r0 + i + NG * lb, L - 1) - u;
+                dma16_s(kb + (size_t)u * k_row2, (uint32_t)l * k_row2 + piece_k, lk + i * S::KG);
+                dma16_s(vb + (size_t)u * v_row2, (uint32_t)l * v_row2 + piece_v, lv + i * S::VG);
+            }
+        }
+    };
+
+    request(0, 0);
+    uint4 qf[NQB][D / 16];
+    int qi[NQB];
+#pragma unroll
+    for (int qb = 0; qb < NQB; qb++) {
+        int hh;
+        split(wrow + 32 * qb + lq, qi[qb], hh);
+        const uint16_t* src = p.q + (size_t)(c0 + qi[qb]) * p.q_row + (size_t)(kvh * p.G + hh) * p.q_head + 8 * lh;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++) qf[qb][kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
+    }
+    f32x16 o[NQB][D / 32];
+    float m[NQB], l[NQB];  // running maximum (log2 units, may lag, below); the lane's own part of the sum
+#pragma unroll
+    for (int qb = 0; qb < NQB; qb++) {
+        m[qb] = -INFINITY;
+        l[qb] = 0.f;
+#pragma unroll
+        for (int db = 0; db < D / 32; db++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[qb][db][r] = 0.f;
+    }
+
+    // Lane addresses in a block of K and V (bytes).
+    const int k_at = (lq % NG) * S::KG + lq / NG * (2 * D) + 16 * (lh ^ S::swap(lq));
+    const int tr_r = 4 * lh + ((lane & 15) >> 2);  // + 16 kk + 8 h: row of the transposing read
+    const int v_at = tr_r % NG * S::VG + tr_r / NG * (2 * D) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    // row + 8 h + 16 kk of the block, from v_at
+    auto v_step = [](int kk, int h) constexpr { return D == 256 ? h * 8 * S::VG + kk * 2 * D : (16 * kk + 8 * h) / NG * 2 * D; };
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    auto v_frag = [&](const char* V, int kk, int db) __attribute__((always_inline)) {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 0) + 64 * db));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 1) + 64 * db));
+        return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    auto compute = [&](int buf, int k0) __attribute__((always_inline)) {
+        const char* K = smem + buf * S::STAGE + k_at;
+        const char* V = smem + buf * S::STAGE + KB * S::KBLK + v_at;
+        f32x16 st[KB][NQB];
+#pragma unroll
+        for (int j = 0; j < KB; j++) {
+#pragma unroll
+            for (int qb = 0; qb < NQB; qb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) st[j][qb][r] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                const uint4 a = *reinterpret_cast<const uint4*>(K + j * S::KBLK + 32 * kk);
+#pragma unroll
+                for (int qb = 0; qb < NQB; qb++) st[j][qb] = E::mfma(a, qf[qb][kk], st[j][qb]);
+            }
+        }
+        bool masked = false;  // uniform: some row of the wave does not attend some key of the tile
+        uint4 pb[KB][NQB][2];
+#pragma unroll
+        for (int qb = 0; qb < NQB; qb++) {
+            const int qfirst = min(wrow + 32 * qb, rows - 1) / p.G;
+            if (k0 + BK - 1 > qfirst) {
+                masked = true;
+#pragma unroll
+                for (int j = 0; j < KB; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (k0 + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3) > qi[qb]) st[j][qb][r] = -INFINITY;
+            }
+            float mx = st[0][qb][0];
+#pragma unroll
+            for (int j = 0; j < KB; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[j][qb][r]);
+            mx = max_xor32(mx) * p.scale2;
+            // The maximum may lag behind by up to 8: weights up to 2^8, all of
+            // a row relative to the same power, so no digit is lost, and the
+            // rescaling of O is skipped in almost every tile.
+            if (__any(mx > m[qb] + 8.f)) {
+                const float mn = fmaxf(m[qb], mx);
+                const float corr = __builtin_amdgcn_exp2f(m[qb] - (mn == -INFINITY ? 0.f : mn));
+                m[qb] = mn;
+                l[qb] *= corr;
+#pragma unroll
+                for (int db = 0; db < D / 32; db++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[qb][db][r] *= corr;
+            }
+            // scores of -inf so far: their weight is 0, not NaN
+            const float base = m[qb] == -INFINITY ? 0.f : m[qb];
+            // P is rounded to the type of the rows, as the matrix units take
+            // it; the sum is of the rounded weights, so they still add up to 1.
+#pragma unroll
+            for (int j = 0; j < KB; j++)
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float s0 = st[j][qb][8 * kk + 2 * i], s1 = st[j][qb][8 * kk + 2 * i + 1];
+                        w[i] = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.scale2, -base)),
+                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.scale2, -base)));
+                        l[qb] = E::dot(w[i], E::ONE, l[qb]);
+                    }
+                    pb[j][qb][kk] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+        }
+        // A weight of 0 times an infinite or NaN value is NaN, so a value that
+        // a row does not attend must not reach its product. Only tiles with
+        // masked keys can hold such a pair; where one of their values is not
+        // finite (bits in `odd`), the product takes 0 for it, and the rows that
+        // do attend it are found by counting: (+inf or NaN) and (-inf or NaN)
+        // entries against the mask, in the same matrix products.
+        uint32_t odd = 0;
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < KB; j++)
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                    for (int db = 0; db < D / 32; db++) {
+                        const uint4 a = v_frag(V + j * S::VBLK, kk, db);
+                        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t e = ~w[i] & E::EXP;  // a half of 0: not finite
+                            odd |= (e & 0xffff) == 0 || (e >> 16) == 0;
+                        }
+                    }
+        }
+        if (__any(odd)) {
+#pragma unroll 1
+            for (int j = 0; j < KB; j++) {
+#pragma unroll
+                for (int qb = 0; qb < NQB; qb++) {
+                    uint4 vis[2];  // 1 where the row attends the key
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = 8 * kk + 2 * i, key = k0 + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3);
+                            w[i] = E::ONE & ((key <= qi[qb] ? 0xffffu : 0u) | (key + 1 <= qi[qb] ? 0xffff0000u : 0u));
+                        }
+                        vis[kk] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+#pragma unroll
+                    for (int db = 0; db < D / 32; db++) {
+                        f32x16 pos, neg;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) pos[r] = neg[r] = 0.f;
+#pragma unroll
+                        for (int kk = 0; kk < 2; kk++) {
+                            const uint4 a = v_frag(V + j * S::VBLK, kk, db);
+                            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                            uint32_t f[4], ip[4], in[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                uint32_t fin = 0, up = 0, dn = 0;
+#pragma unroll
+                                for (int hf = 0; hf < 2; hf++) {
+                                    const uint32_t sel = 0xffffu << (16 * hf), y = w[i] & sel;
+                                    const bool bad = (y & E::EXP) == (E::EXP & sel), nan = bad && (y & E::MANT);
+                                    const bool sign = (y >> (16 * hf + 15)) & 1;
+                                    if (!bad) fin |= y;
+                                    if (bad && (nan || !sign)) up |= E::ONE & sel;
+                                    if (bad && (nan || sign)) dn |= E::ONE & sel;
+                                }
+                                f[i] = fin;
+                                ip[i] = up;
+                                in[i] = dn;
+                            }
+                            const uint4 pj = j == 0 || KB == 1 ? pb[0][qb][kk] : pb[KB - 1][qb][kk];
+                            o[qb][db] = E::mfma(make_uint4(f[0], f[1], f[2], f[3]), pj, o[qb][db]);
+                            pos = E::mfma(make_uint4(ip[0], ip[1], ip[2], ip[3]), vis[kk], pos);
+                            neg = E::mfma(make_uint4(in[0], in[1], in[2], in[3]), vis[kk], neg);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            if (pos[r] > 0.f) o[qb][db][r] += INFINITY;
+                            if (neg[r] > 0.f) o[qb][db][r] -= INFINITY;
+                        }
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < KB; j++)
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                    for (int db = 0; db < D / 32; db++) {
+                        const uint4 a = v_frag(V + j * S::VBLK, kk, db);
+#pragma unroll
+                        for (int qb = 0; qb < NQB; qb++) o[qb][db] = E::mfma(a, pb[j][qb][kk], o[qb][db]);
+                    }
+        }
+    };
+
+    // Two stages: step i requests tile i + 1 into the stage that the barrier
+    // before it freed, computes tile i, waits for its own requests, and the
+    // barrier publishes tile i + 1.
+    wait_vm<0>();
+    __syncthreads();
+    for (int it = 0, buf = 0; it < ntiles; it++, buf ^= 1) {
+        const int k0 = it * BK;
+        const bool more = it + 1 < ntiles;
+        if (more) request(k0 + BK, buf ^ 1);
+        if (k0 <= last) compute(buf, k0);
+        if (more) {
+            wait_vm<0>();
+            __syncthreads();
+        }
+    }
+
+    // Rows out: the wave's 32 columns are 32 rows, a lane holding 4-dim pieces
+    // of one, so they go through LDS (64 dims a pass, f32: the one rounding
+    // comes after the gate) and leave as 16-byte pieces, 8 lanes per row.
+    __syncthreads();  // every wave is past the last tile's stage
+    float* ew = reinterpret_cast<float*>(smem) + wave * 32 * S::RR;
+    const int er = lane >> 3, ec = lane & 7;
+#pragma unroll
+    for (int qb = 0; qb < NQB; qb++) {
+        const float inv = 1.f / add_xor32(l[qb]);
+        size_t t[4];
+        int head[4];
+        bool ok[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int r = wrow + 32 * qb + er + 8 * k;
+            int qq, hh;
+            split(r, qq, hh);
+            ok[k] = r < rows;
+            t[k] = (size_t)(c0 + qq);
+            head[k] = kvh * p.G + hh;
+        }
+#pragma unroll
+        for (int ps = 0; ps < D / 64; ps++) {
+#pragma unroll
+            for (int db = 2 * ps; db < 2 * ps + 2; db++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f32x16& y = o[qb][db];
+                    *reinterpret_cast<float4*>(ew + lq * S::RR + 32 * (db - 2 * ps) + 8 * g + 4 * lh) =
+                        make_float4(y[4 * g] * inv, y[4 * g + 1] * inv, y[4 * g + 2] * inv, y[4 * g + 3] * inv);
+                }
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float* src = ew + (er + 8 * k) * S::RR + 8 * ec;
+                const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+                float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                if (p.gate) {
+                    const uint4 g = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head +
+                                                                    64 * ps + 8 * ec);
+                    const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        y[2 * i] = gated_div(y[2 * i], 1.f + __expf(-E::lo(gw[i])));
+                        y[2 * i + 1] = gated_div(y[2 * i + 1], 1.f + __expf(-E::hi(gw[i])));
+                    }
+                }
+                if (ok[k])
+                    *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + 64 * ps + 8 * ec) =
+                        make_uint4(E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7]));
+            }
+            wave_sync();  // the region is rewritten by the next pass
+        }
+    }
+}
+
+// 1-D grid of at least (tiles of the batch) x Hkv workgroups, kv heads first:
+// workgroup ids go to the 8 XCDs in turn, so with 1, 2, 4 or a multiple of 8
+// kv heads an XCD reads the K and V of few heads through its L2.
+template <class E, int D, int NQB, int KB, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) packed_kernel(PackedParams p) {
+    using S = PackedTile<D, NQB, KB, NW>;
+    __shared__ __align__(16) char smem[S::LDS];
+    const int kvh = blockIdx.x % p.Hkv;
+    int c0, n, x;
+    if (!find_packed_tile<S::RW, NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
+    packed_tile<E, D, NQB, KB, NW>(p, smem, c0, n, x, kvh);
+}
+
+}  // namespace pkv

@@ -1,0 +1,273 @@
+"""Attention over packed prompts (pkv.attn_packed) against the formula in 64
+bits, on the GPU.
+
+Bound per element, from the kernel's arithmetic with u half a step of the row
+type (2^-8 bf16, 2^-11 fp16) and A = sum_j w_j |v_j| of the softmax weights w:
+  u A         the weights rounded for the second product
+  u |out|     their sum (of the same rounded weights), u |out| the output's own rounding; below the type's smallest
+              normal number (2^-14 in fp16) the spacing stays that number's: u times it (2^-25)
+  e (A + |out|)   scores in f32: a dot product of D terms is off by at most (D + 16) 2^-24 scale sum |q k|
+              (S, its largest over the row's keys), twice that in a ratio of weights, and 2^-20 for exp2, the
+              sigmoid and the division
+  n 2^-24 A   n weighted values added up in f32
+  fp16: weights below 2^-14 are multiples of 2^-24, off by 2^-25 at most: n 2^-25 max |v| (the largest weight is 1
+        or more).
+"""
+import numpy as np
+import pytest
+import torch
+
+import pkv
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def offsets(lens, lead=0):
+    return np.concatenate([[lead], lead + np.cumsum(lens)]).astype(np.int32)
+
+
+def inputs(lens, Hq, Hkv, D, dtype, seed, dev, gate=False, lead=0, tail=0, amp=1.5):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    T = int(sum(lens)) + lead + tail
+    r = lambda H, a: (torch.randn(T, H, D, device=dev, generator=g) * a).to(TYPES[dtype])
+    return dict(q=r(Hq, amp), k=r(Hkv, amp), v=r(Hkv, 1.0), gate=r(Hq, 2.0) if gate else None,
+                cu=torch.from_numpy(offsets(lens, lead)).to(dev), lens=list(lens), lead=lead, scale=D ** -0.5)
+
+
+def reference(c):
+    """out and its bound in float64, rows outside the sequences NaN."""
+    q, k, v = (c[n].double() for n in ("q", "k", "v"))
+    T, Hq, D = q.shape
+    G = Hq // k.shape[1]
+    u = torch.finfo(c["q"].dtype).eps / 2
+    out = torch.full((T, Hq, D), float("nan"), dtype=torch.float64, device=q.device)
+    tol = out.clone()
+    a = c["lead"]
+    for n in c["lens"]:
+        for h in range(Hq if n else 0):
+            qq, kk, vv = q[a:a + n, h], k[a:a + n, h // G], v[a:a + n, h // G]
+            seen = torch.ones(n, n, dtype=torch.bool, device=q.device).tril()
+            x = torch.where(seen, qq @ kk.t().contiguous() * c["scale"], -float("inf"))
+            w = torch.softmax(x, -1)
+            o, A = w @ vv, w @ vv.abs()
+            S = torch.where(seen, qq.abs() @ kk.abs().t().contiguous() * c["scale"], 0).amax(-1, keepdim=True)
+            e = 2 * (D + 16) * 2.0 ** -24 * S + 2.0 ** -20
+            m = torch.arange(1, n + 1, device=q.device, dtype=torch.float64)[:, None]
+            low = m * 2.0 ** -25 * vv.abs().amax() if c["q"].dtype is torch.float16 else 0
+            t = (u + e + m * 2.0 ** -24) * A + (u + e) * o.abs() + low
+            sig = torch.sigmoid(c["gate"][a:a + n, h].double()) if c["gate"] is not None else 1.0
+            out[a:a + n, h] = o * sig
+            tol[a:a + n, h] = t * sig + u * (o * sig).abs() + torch.finfo(c["q"].dtype).tiny * u
+        a += n
+    return out, tol
+
+
+def run(c, out=None, **kw):
+    if out is None:
+        out = torch.full_like(c["q"], 7.0)
+    pkv.attn_packed(c["q"], c["k"], c["v"], c["cu"], out, c["scale"], gate=c["gate"], **kw)
+    return out
+
+
+def check(c, got, what=""):
+    want, tol = reference(c)
+    rows = slice(c["lead"], c["lead"] + sum(c["lens"]))
+    err = (got[rows].double() - want[rows]).abs()
+    worst = float((err / tol[rows]).max()) if err.numel() else 0.0
+    print(f"{what}: {err.numel()} elements, worst error over bound {worst:.3f}", flush=True)
+    assert worst <= 1.0 and not torch.isnan(got[rows]).any()
+
+
+LENS = [[1], [2, 1, 0, 5], [31, 32, 33, 0], [63, 64, 65, 127, 128, 129], [300, 1, 700], [1025]]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (6, 6), (14, 2), (20, 4)])
+def test_rows_match_the_formula(dev, dtype, D, Hq, Hkv):
+    for i, lens in enumerate(LENS):
+        print("case", dtype, D, Hq, Hkv, lens, flush=True)
+        c = inputs(lens, Hq, Hkv, D, dtype, 100 * i + D + Hq, dev, gate=i % 2 == 1)
+        check(c, run(c), f"{dtype} D {D} heads {Hq}/{Hkv} lens {lens}")
+
+
+@pytest.mark.parametrize("G", [1, 2, 3, 5, 8, 16, 40])
+def test_any_group(dev, G):
+    print("case group", G, flush=True)
+    c = inputs([77, 130, 3], 2 * G, 2, 64, "bf16", G, dev)
+    check(c, run(c), f"G {G}")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_prompts_and_many_sequences(dev, D):
+    for lens, Hq, Hkv in (([5000], 2, 1), ([1 + 7 * i % 50 for i in range(700)], 4, 2)):
+        print("case", D, len(lens), flush=True)
+        c = inputs(lens, Hq, Hkv, D, "bf16", D, dev)
+        check(c, run(c), f"D {D}, {len(lens)} sequences")
+
+
+def test_views_of_a_projection_row(dev):
+    """q and gate inside [Hq x (q | gate) | k | v] rows, out head-major and inside wider rows."""
+    lens, Hq, Hkv, D = [40, 100, 7], 8, 2, 128
+    T = sum(lens)
+    x = (torch.randn(T, (2 * Hq + 2 * Hkv) * D, device=dev, generator=torch.Generator(dev).manual_seed(3))).bfloat16()
+    qg = x[:, :2 * Hq * D].view(T, Hq, 2, D)
+    c = dict(q=qg[:, :, 0], gate=qg[:, :, 1], k=x[:, 2 * Hq * D:(2 * Hq + Hkv) * D].view(T, Hkv, D),
+             v=x[:, (2 * Hq + Hkv) * D:].view(T, Hkv, D), cu=torch.from_numpy(offsets(lens)).to(dev), lens=lens, lead=0,
+             scale=D ** -0.5)
+    major = torch.full((Hq, T, D), 7.0, device=dev, dtype=torch.bfloat16)
+    run(c, major.transpose(0, 1))
+    check(c, major.transpose(0, 1), "head-major out")
+    wide = torch.full((T, Hq, 3, D), 7.0, device=dev, dtype=torch.bfloat16)
+    run(c, wide[:, :, 1])
+    assert torch.equal(wide[:, :, 1], major.transpose(0, 1)) and (wide[:, :, 0::2] == 7).all()
+    # one kv head for all, by a stride of 0
+    c["k"], c["v"] = c["k"][:, :1].expand(T, 2, D), c["v"][:, :1].expand(T, 2, D)
+    check(c, run(c), "broadcast kv heads")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_outside_the_sequences(dev, D):
+    """Rows before the first and behind the last sequence, NaN in them: neither read into others nor written."""
+    c = inputs([70, 0, 33], 4, 2, D, "bf16", 5, dev, gate=True, lead=9, tail=50)
+    inner = slice(9, 9 + 103)
+    clean = run(c)
+    for n in ("q", "k", "v", "gate"):
+        keep = c[n][inner].clone()
+        c[n].fill_(float("nan"))
+        c[n][inner] = keep
+    got = run(c)
+    assert torch.equal(got[inner], clean[inner])
+    assert (got[:9] == 7).all() and (got[9 + 103:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_infinite_and_nan_values_reach_the_rows_that_attend_them(dev, D, dtype):
+    lens, Hq, Hkv = [150, 40], 6, 2
+    c = inputs(lens, Hq, Hkv, D, dtype, 11, dev)
+    clean = run(c)
+    inf = float("inf")
+    for at, x in ((3, inf), (37, -inf), (38, float("nan")), (100, inf), (101, -inf), (149, float("nan"))):
+        y = dict(c, v=c["v"].clone())
+        y["v"][at, 1, 5] = x
+        got = run(y)
+        # what does not attend it: earlier rows, the other sequence, other kv heads and dims
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[at:150, 3:, 5] = False
+        assert torch.equal(got[same], clean[same]), (at, x)
+        hit = got[at:150, 3:, 5]
+        # (an fp16 weight below 2^-25 is 0, and 0 x infinity NaN)
+        assert (torch.isnan(hit) if x != x else (hit == x) | (torch.isnan(hit) & (dtype == "fp16"))).all(), (at, x)
+    # both signs: NaN from the row on that attends both
+    y = dict(c, v=c["v"].clone())
+    y["v"][100, 0, 0], y["v"][101, 0, 0] = inf, -inf
+    got = run(y)
+    assert not torch.isfinite(got[100, :3, 0]).any() and torch.isnan(got[101:150, :3, 0]).all()
+    assert torch.equal(got[:100], clean[:100])
+    # keys: a NaN key makes the rows that attend it NaN, an infinite one decides or drops out
+    y = dict(c, k=c["k"].clone())
+    y["k"][60, 0] = float("nan")
+    got = run(y)
+    assert torch.equal(got[:60], clean[:60]) and torch.isnan(got[60:150, :3]).all()
+    assert torch.equal(got[:, 3:], clean[:, 3:]) and torch.equal(got[150:], clean[150:])
+    # a query: its own row
+    y = dict(c, q=c["q"].clone())
+    y["q"][20, 2, 0] = inf
+    got = run(y)
+    same = torch.ones(got.shape[:2], dtype=torch.bool, device=dev)
+    same[20, 2] = False
+    assert torch.equal(got[same], clean[same])
+
+
+def test_scores_of_minus_infinity_first(dev):
+    """The first keys score -inf for every row: weight 0 once another key does not; alone, the formula's NaN."""
+    c = inputs([100], 2, 1, 64, "bf16", 2, dev)
+    c["q"][:, :, 0] = 1.0
+    c["k"][:40, :, 0] = -float("inf")
+    c["k"][40:, :, 0] = 0.0
+    got = run(c)
+    assert torch.isnan(got[:40]).all()
+    # the same rows without those keys
+    x = dict(c, q=c["q"][40:], k=c["k"][40:], v=c["v"][40:], cu=torch.tensor([0, 60], dtype=torch.int32, device=dev),
+             lens=[60])
+    check(x, got[40:], "behind 40 keys of -inf")
+
+
+@pytest.mark.parametrize("amp", [0.0, 30.0])
+def test_flat_and_extreme_scores(dev, amp):
+    """All scores equal, and scores of hundreds that leave one key."""
+    c = inputs([200, 65], 4, 2, 128, "bf16", 8, dev, amp=amp)
+    check(c, run(c), f"amp {amp}")
+
+
+def test_rising_scores(dev):
+    """Every key scores above the ones before: the running maximum moves at every tile."""
+    for D, step in ((64, 0.02), (128, 0.5), (256, 3.0)):
+        c = inputs([600], 2, 2, D, "bf16", D, dev)
+        c["q"][:] = 1.0
+        c["k"][:] = (torch.arange(600, device=dev) * step / D * D ** 0.5)[:, None, None].to(torch.bfloat16)
+        check(c, run(c), f"D {D} step {step}")
+
+
+def test_offsets_out_of_range_are_clamped(dev):
+    c = inputs([50, 30], 2, 1, 64, "bf16", 4, dev)
+    want = run(c)
+    y = dict(c, cu=torch.tensor([0, 50, 1 << 30], dtype=torch.int32, device=dev))
+    assert torch.equal(run(y), want)
+    y = dict(c, cu=torch.tensor([-7, 50, 80], dtype=torch.int32, device=dev))
+    assert torch.equal(run(y), want)
+    # offsets that go back: an empty sequence
+    y = dict(c, cu=torch.tensor([0, 50, 20, 20], dtype=torch.int32, device=dev))
+    got = run(y)
+    assert torch.equal(got[:50], want[:50]) and (got[50:] == 7).all()
+
+
+def test_no_rows(dev):
+    c = inputs([5], 2, 1, 64, "bf16", 4, dev)
+    empty = dict(c, cu=c["cu"][:1])
+    assert (run(empty) == 7).all()
+    none = {n: c[n][:0] if n in ("q", "k", "v") else c[n] for n in c}
+    assert run(none).numel() == 0
+
+
+def test_captured_and_replayed(dev):
+    """One graph for a batch of 300 rows and up to 4 prompts, replayed over new lengths and values, eager calls between."""
+    c = inputs([100, 200], 6, 2, 128, "bf16", 1, dev)
+    c["cu"] = torch.tensor([0, 100, 300, 300, 300], dtype=torch.int32, device=dev)
+    out = torch.zeros_like(c["q"])
+    run(c, out)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        run(c, out)
+    for i, lens in enumerate(([100, 200], [1, 1, 1, 297], [300], [40, 0, 64])):
+        new = inputs(lens, 6, 2, 128, "bf16", 50 + i, dev, tail=300 - sum(lens))
+        for n in ("q", "k", "v"):
+            c[n].copy_(new[n])
+        cu = offsets(lens)
+        c["cu"].copy_(torch.from_numpy(np.concatenate([cu, np.full(5 - len(cu), cu[-1])]).astype(np.int32)))
+        out.fill_(7.0)
+        graph.replay()
+        want = run(dict(c))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), lens
+        check(dict(new, cu=c["cu"]), out, f"replay {lens}")
+
+
+def test_two_streams_and_repeats(dev):
+    """Calls on two streams at once, no workspace between them, and the same bits every time."""
+    cases = [inputs([400, 90], 8, 2, 128, "bf16", 1, dev), inputs([33, 257], 8, 2, 256, "fp16", 2, dev, gate=True)]
+    want = [run(c) for c in cases]
+    outs = [torch.zeros_like(c["q"]) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(10):
+        for c, o, s in zip(cases, outs, streams):
+            run(c, o, stream=s)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
