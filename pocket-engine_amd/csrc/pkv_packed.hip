@@ -22,6 +22,14 @@
 
 namespace pkv {
 
+// 1 / (1 + e^-g) with e^-|g| as a square, so that it reaches f32's subnormal
+// numbers (gates down to -103 keep their order of magnitude) and nothing
+// overflows.
+__device__ __forceinline__ float sigmoid(float g) {
+    const float h = __builtin_amdgcn_exp2f(-0.5f * LOG2E * __builtin_fabsf(g)), e = h * h;
+    return (g < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+}
+
 struct PackedParams {
     const uint16_t *q, *k, *v, *gate;  // gate: null for none
     uint16_t* out;
@@ -114,8 +122,10 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
     return true;
 }
 
+// `odd`: 2 D + 1 words: per dim the first keys with values that are not finite
+// (tame, below), and whether there are any.
 template <class E, int D, int NQB, int KB, int NW>
-__device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, int c0, int n, int x, int kvh) {
+__device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, int* odd, int c0, int n, int x, int kvh) {
     using S = PackedTile<D, NQB, KB, NW>;
     constexpr int NG = S::NG, BK = S::BK;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lq = lane & 31,
@@ -170,6 +180,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     };
 
     request(0, 0);
+    for (int i = tid; i <= 2 * D; i += S::THREADS) odd[i] = i < 2 * D ? 0x7fffffff : 0;
     uint4 qf[NQB][D / 16];
     int qi[NQB];
 #pragma unroll
@@ -222,13 +233,11 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                 for (int qb = 0; qb < NQB; qb++) st[j][qb] = E::mfma(a, qf[qb][kk], st[j][qb]);
             }
         }
-        bool masked = false;  // uniform: some row of the wave does not attend some key of the tile
         uint4 pb[KB][NQB][2];
 #pragma unroll
         for (int qb = 0; qb < NQB; qb++) {
             const int qfirst = min(wrow + 32 * qb, rows - 1) / p.G;
             if (k0 + BK - 1 > qfirst) {
-                masked = true;
 #pragma unroll
                 for (int j = 0; j < KB; j++)
 #pragma unroll
@@ -273,102 +282,63 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                     pb[j][qb][kk] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
         }
-        // A weight of 0 times an infinite or NaN value is NaN, so a value that
-        // a row does not attend must not reach its product. Only tiles with
-        // masked keys can hold such a pair; where one of their values is not
-        // finite (bits in `odd`), the product takes 0 for it, and the rows that
-        // do attend it are found by counting: (+inf or NaN) and (-inf or NaN)
-        // entries against the mask, in the same matrix products.
-        uint32_t odd = 0;
-        if (masked) {
 #pragma unroll
-            for (int j = 0; j < KB; j++)
+        for (int j = 0; j < KB; j++)
 #pragma unroll
-                for (int kk = 0; kk < 2; kk++)
+            for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-                    for (int db = 0; db < D / 32; db++) {
-                        const uint4 a = v_frag(V + j * S::VBLK, kk, db);
-                        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                for (int db = 0; db < D / 32; db++) {
+                    const uint4 a = v_frag(V + j * S::VBLK, kk, db);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t e = ~w[i] & E::EXP;  // a half of 0: not finite
-                            odd |= (e & 0xffff) == 0 || (e >> 16) == 0;
-                        }
-                    }
-        }
-        if (__any(odd)) {
-#pragma unroll 1
-            for (int j = 0; j < KB; j++) {
-#pragma unroll
-                for (int qb = 0; qb < NQB; qb++) {
-                    uint4 vis[2];  // 1 where the row attends the key
-#pragma unroll
-                    for (int kk = 0; kk < 2; kk++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r = 8 * kk + 2 * i, key = k0 + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3);
-                            w[i] = E::ONE & ((key <= qi[qb] ? 0xffffu : 0u) | (key + 1 <= qi[qb] ? 0xffff0000u : 0u));
-                        }
-                        vis[kk] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-#pragma unroll
-                    for (int db = 0; db < D / 32; db++) {
-                        f32x16 pos, neg;
-#pragma unroll
-                        for (int r = 0; r < 16; r++) pos[r] = neg[r] = 0.f;
-#pragma unroll
-                        for (int kk = 0; kk < 2; kk++) {
-                            const uint4 a = v_frag(V + j * S::VBLK, kk, db);
-                            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-                            uint32_t f[4], ip[4], in[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                uint32_t fin = 0, up = 0, dn = 0;
-#pragma unroll
-                                for (int hf = 0; hf < 2; hf++) {
-                                    const uint32_t sel = 0xffffu << (16 * hf), y = w[i] & sel;
-                                    const bool bad = (y & E::EXP) == (E::EXP & sel), nan = bad && (y & E::MANT);
-                                    const bool sign = (y >> (16 * hf + 15)) & 1;
-                                    if (!bad) fin |= y;
-                                    if (bad && (nan || !sign)) up |= E::ONE & sel;
-                                    if (bad && (nan || sign)) dn |= E::ONE & sel;
-                                }
-                                f[i] = fin;
-                                ip[i] = up;
-                                in[i] = dn;
-                            }
-                            const uint4 pj = j == 0 || KB == 1 ? pb[0][qb][kk] : pb[KB - 1][qb][kk];
-                            o[qb][db] = E::mfma(make_uint4(f[0], f[1], f[2], f[3]), pj, o[qb][db]);
-                            pos = E::mfma(make_uint4(ip[0], ip[1], ip[2], ip[3]), vis[kk], pos);
-                            neg = E::mfma(make_uint4(in[0], in[1], in[2], in[3]), vis[kk], neg);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            if (pos[r] > 0.f) o[qb][db][r] += INFINITY;
-                            if (neg[r] > 0.f) o[qb][db][r] -= INFINITY;
-                        }
-                    }
+                    for (int qb = 0; qb < NQB; qb++) o[qb][db] = E::mfma(a, pb[j][qb][kk], o[qb][db]);
                 }
+    };
+
+    // A weight of 0 times an infinite or NaN value is NaN, so a value must not
+    // meet the weights of rows that do not attend its key. Only tiles with
+    // keys behind the tile's first query can hold such a pair: there the wave
+    // looks through the values that it brought, takes out what is not finite,
+    // and notes for its dim the first key with (+inf or NaN) and with (-inf or
+    // NaN). A row attends a key if and only if the key is not behind it, so
+    // those two say what the finished rows get.
+    const int first_q = row0 / p.G;
+    auto tame = [&](int k0, int buf) __attribute__((always_inline)) {
+        if (k0 + BK - 1 <= first_q) return;
+#pragma unroll
+        for (int i = 0; i < S::PER; i++) {
+            uint4* at = reinterpret_cast<uint4*>(smem + buf * S::STAGE + KB * S::KBLK + j0 * S::VBLK + (g0 + i) * S::VG +
+                                                 16 * lane);
+            const uint4 x = *at;
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t u = ~w[e] & E::EXP;  // a half of 0: not finite
+                bad |= (u & 0xffffu) == 0 || (u >> 16) == 0;
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < KB; j++)
-#pragma unroll
-                for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                    for (int db = 0; db < D / 32; db++) {
-                        const uint4 a = v_frag(V + j * S::VBLK, kk, db);
-#pragma unroll
-                        for (int qb = 0; qb < NQB; qb++) o[qb][db] = E::mfma(a, pb[j][qb][kk], o[qb][db]);
-                    }
+            if (bad) {
+                const int key = k0 + 32 * j0 + g0 + i + NG * lb;
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t y = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                    if ((~y & E::EXP & 0xffffu) != 0) continue;
+                    const bool nan = y & E::MANT & 0xffffu, minus = y >> 15;
+                    if (nan || !minus) atomicMin(odd + 8 * lc + e, key);
+                    if (nan || minus) atomicMin(odd + D + 8 * lc + e, key);
+                    w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
+                }
+                *at = make_uint4(w[0], w[1], w[2], w[3]);
+                odd[2 * D] = 1;
+            }
         }
     };
 
     // Two stages: step i requests tile i + 1 into the stage that the barrier
     // before it freed, computes tile i, waits for its own requests, and the
     // barrier publishes tile i + 1.
+    __syncthreads();  // `odd` is set
     wait_vm<0>();
+    tame(0, 0);
     __syncthreads();
     for (int it = 0, buf = 0; it < ntiles; it++, buf ^= 1) {
         const int k0 = it * BK;
@@ -377,6 +347,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         if (k0 <= last) compute(buf, k0);
         if (more) {
             wait_vm<0>();
+            tame(k0 + BK, buf ^ 1);
             __syncthreads();
         }
     }
@@ -387,11 +358,12 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     __syncthreads();  // every wave is past the last tile's stage
     float* ew = reinterpret_cast<float*>(smem) + wave * 32 * S::RR;
     const int er = lane >> 3, ec = lane & 7;
+    const bool any_odd = odd[2 * D] != 0;
 #pragma unroll
     for (int qb = 0; qb < NQB; qb++) {
         const float inv = 1.f / add_xor32(l[qb]);
         size_t t[4];
-        int head[4];
+        int head[4], query[4];
         bool ok[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -400,6 +372,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
             split(r, qq, hh);
             ok[k] = r < rows;
             t[k] = (size_t)(c0 + qq);
+            query[k] = qq;
             head[k] = kvh * p.G + hh;
         }
 #pragma unroll
@@ -418,14 +391,21 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                 const float* src = ew + (er + 8 * k) * S::RR + 8 * ec;
                 const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
                 float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                if (any_odd) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (query[k] >= odd[64 * ps + 8 * ec + i]) y[i] += INFINITY;
+                        if (query[k] >= odd[D + 64 * ps + 8 * ec + i]) y[i] -= INFINITY;
+                    }
+                }
                 if (p.gate) {
                     const uint4 g = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head +
                                                                     64 * ps + 8 * ec);
                     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        y[2 * i] = gated_div(y[2 * i], 1.f + __expf(-E::lo(gw[i])));
-                        y[2 * i + 1] = gated_div(y[2 * i + 1], 1.f + __expf(-E::hi(gw[i])));
+                        y[2 * i] *= sigmoid(E::lo(gw[i]));
+                        y[2 * i + 1] *= sigmoid(E::hi(gw[i]));
                     }
                 }
                 if (ok[k])
@@ -444,10 +424,11 @@ template <class E, int D, int NQB, int KB, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) packed_kernel(PackedParams p) {
     using S = PackedTile<D, NQB, KB, NW>;
     __shared__ __align__(16) char smem[S::LDS];
+    __shared__ int odd[2 * D + 1];
     const int kvh = blockIdx.x % p.Hkv;
     int c0, n, x;
     if (!find_packed_tile<S::RW, NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
-    packed_tile<E, D, NQB, KB, NW>(p, smem, c0, n, x, kvh);
+    packed_tile<E, D, NQB, KB, NW>(p, smem, odd, c0, n, x, kvh);
 }
 
 }  // namespace pkv

@@ -182,6 +182,23 @@ def test_infinite_and_nan_values_reach_the_rows_that_attend_them(dev, D, dtype):
     assert torch.equal(got[same], clean[same])
 
 
+def test_gates_at_their_ends(dev):
+    """Gates that close a row (down to the smallest results), open it, are infinite or NaN, and one on an infinite value."""
+    c = inputs([60], 4, 2, 64, "bf16", 12, dev, gate=True)
+    ends = torch.tensor([-87.0, -87.5, -88.5, -100.0, -30.0, 0.0, 20.0, 88.0, 3e38], device=dev).bfloat16()
+    c["gate"][:, :, :9] = ends
+    plain = run(dict(c, gate=None))
+    got = run(c)
+    check(c, got, "gates")
+    # (0.01 e^-87 is above 2^-133, the smallest number)
+    assert (got[:, :, 0] != 0)[plain[:, :, 0].abs() > 0.01].all() and torch.equal(got[:, :, 8], plain[:, :, 8])
+    c["gate"][:, :, 0], c["gate"][:, :, 1], c["gate"][:, :, 2] = -float("inf"), float("inf"), float("nan")
+    c["v"][30, 0, 5] = float("inf")
+    got = run(c)
+    assert (got[:, :, 0] == 0).all() and torch.equal(got[:, :, 1], plain[:, :, 1]) and torch.isnan(got[:, :, 2]).all()
+    assert (got[30:, :2, 5] == float("inf")).all()
+
+
 def test_scores_of_minus_infinity_first(dev):
     """The first keys score -inf for every row: weight 0 once another key does not; alone, the formula's NaN."""
     c = inputs([100], 2, 1, 64, "bf16", 2, dev)
