@@ -22,12 +22,10 @@
 
 namespace pkv {
 
-// 1 / (1 + e^-g) with e^-|g| as a square, so that it reaches f32's subnormal
-// numbers (gates down to -103 keep their order of magnitude) and nothing
-// overflows.
+// 1 / (1 + e^-g); 0 for gates below -87.3, where e^-g passes the reciprocal's
+// normal results (the value there is below 1.2e-38).
 __device__ __forceinline__ float sigmoid(float g) {
-    const float h = __builtin_amdgcn_exp2f(-0.5f * LOG2E * __builtin_fabsf(g)), e = h * h;
-    return (g < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * g));
 }
 
 struct PackedParams {
@@ -41,10 +39,12 @@ struct PackedParams {
 };
 
 // Shapes of a workgroup: D dims a head, NW waves of 32 NQB rows, tiles of KB
-// blocks of 32 keys, two stages.
-template <int D, int NQB, int KB, int NW>
+// blocks of 32 keys, NST stages. SPLIT: the waves have the same 32 NQB rows and
+// take the key tiles in turn, each through stages of its own, and the waves'
+// sums are joined at the end.
+template <int D, int NQB, int KB, int NW, int NST = 2, bool SPLIT = false>
 struct PackedTile {
-    static constexpr int RW = 32 * NQB * NW, BK = 32 * KB, THREADS = 64 * NW;
+    static constexpr int RW = 32 * NQB * (SPLIT ? 1 : NW), BK = 32 * KB, THREADS = 64 * NW;
     // A 32-row block of K or V in LDS: NG groups of 1,024 bytes, one LDS DMA
     // instruction each; row r lies in group r % NG at (r / NG) 2 D bytes.
     // K groups are 1,056 bytes apart (1,040 at 256 dims) and rows with bit 3
@@ -56,40 +56,126 @@ struct PackedTile {
     static constexpr int KG = D == 256 ? 1040 : 1056, VG = 1088;
     static constexpr int KBLK = NG * KG, VBLK = NG * VG;
     static constexpr int STAGE = KB * (KBLK + VBLK);
-    static constexpr int PER = KB * NG / NW;  // groups of K (and of V) that a wave requests per tile
+    static constexpr int PER = KB * NG / (SPLIT ? 1 : NW);  // groups of K (and of V) that a wave requests per tile
     static constexpr int RR = 68;             // staged output row, floats of 64 dims
     static constexpr int EPI = NW * 32 * RR * 4;
-    static constexpr int LDS = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+    static constexpr int STAGES = NST * (SPLIT ? NW : 1) * STAGE;
+    static constexpr int LDS = STAGES > EPI ? STAGES : EPI;
     static_assert(KB * NG % NW == 0 && NG % PER == 0, "a wave's groups lie in one block");
+    static_assert(NST == 2 || (SPLIT && NST == 1), "two stages, or one per wave");
+    static_assert(!SPLIT || NQB == 1, "32 rows");
     static __device__ __forceinline__ constexpr int swap(int r) { return D == 256 ? 0 : (r >> 3) & 1; }
 };
 
-// Sequence s and its tile x of this workgroup among the batch's tiles, numbered
-// from the last: later tiles of a sequence attend more keys, so the longest
-// work is started first. Each thread counts the tiles of `per` sequences, the
-// prefix sums over threads find the one that holds the tile. False where the
-// grid has more workgroups than the batch has tiles.
+// Reductions and the inclusive prefix sum over the wave's lanes by row moves.
+template <class Op>
+__device__ __forceinline__ int wave_all(int v, Op op) {
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR1, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, DPP_QUAD_XOR2, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, DPP_ROW_HALF_MIRROR, 0xf, 0xf, false));
+    v = op(v, __builtin_amdgcn_update_dpp(0, v, DPP_ROW_MIRROR, 0xf, 0xf, false));
+    auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, true, false);
+    v = op((int)r[0], (int)r[1]);
+    r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, true, false);
+    return __builtin_amdgcn_readfirstlane(op((int)r[0], (int)r[1]));
+}
+__device__ __forceinline__ int wave_sum(int v) {
+    return wave_all(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_max(int v) {
+    return wave_all(v, [](int a, int b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111 /* row_shr:1 */, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112 /* row_shr:2 */, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114 /* row_shr:4 */, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118 /* row_shr:8 */, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142 /* row_bcast:15 */, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143 /* row_bcast:31 */, 0xc, 0xf, false);
+    return v;
+}
+
+// This workgroup's sequence (rows c0 .. c0 + n - 1) and its tile x of it. False
+// where the grid has more workgroups than the batch has tiles. A tile x of any
+// sequence attends up to (x + 1) RW / G keys, so the order of the tiles is the
+// order of their work, and the longest are started first, whatever the
+// sequences' order (LEVEL_SEQS sequences or fewer): with c_s tiles in sequence
+// s, N(j) = sum_s max(0, c_s - j) tiles have x >= j, so the tile of rank r has
+// the largest x with N(x) > r, found by halving. Every wave does it for
+// itself, 4 sequences to a lane, without LDS or barriers (about 0.5 us beside
+// the offsets' load). More sequences: last sequence first, the tiles of each
+// from the last, by a prefix sum over the workgroup's threads.
+constexpr int LEVEL_SEQS = 256;
 template <int RW, int NW>
 __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile, int& c0, int& n, int& x) {
-    __shared__ int wsum[NW], found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (p.seqs + 64 * NW - 1) / (64 * NW);
-    const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
     // offsets outside [0, T] are clamped: no row out of range is touched
     auto at = [&](int s) { return max(0, min(p.cu[s], p.T)); };
     auto tiles = [&](int a, int b) { return b > a ? ((b - a) * p.G + RW - 1) / RW : 0; };
+    if (p.seqs == 1) {
+        c0 = at(0);
+        n = at(1) - c0;
+        x = tiles(c0, c0 + n) - 1 - tile;
+        return x >= 0;
+    }
+    if (p.seqs <= LEVEL_SEQS) {
+        int off[5], c[4], most = 0, sum = 0;
+#pragma unroll
+        for (int i = 0; i < 5; i++) off[i] = at(min(4 * lane + i, p.seqs));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[i] = tiles(off[i], off[i + 1]);
+            most = max(most, c[i]);
+            sum += c[i];
+        }
+        const int total = wave_sum(sum);
+        if (tile >= total) return false;
+        auto above = [&](int j) {
+            int k = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) k += max(0, c[i] - j);
+            return wave_sum(k);
+        };
+        int lo = 0, hi = wave_max(most) - 1, after = 0;  // N(lo) > tile; after = N(hi + 1)
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1, k = above(mid);
+            if (k > tile) {
+                lo = mid;
+            } else {
+                hi = mid - 1;
+                after = k;
+            }
+        }
+        // the (tile - N(x + 1))-th sequence that has a tile x
+        int k = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) k += c[i] > lo;
+        const int incl = wave_prefix(k);
+        int r = tile - after - (incl - k), a = 0, b = 0;
+        const unsigned long long hit = __ballot(r >= 0 && r < k);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (c[i] > lo && r-- == 0) {
+                a = off[i];
+                b = off[i + 1];
+            }
+        }
+        const int l = __ffsll((long long)hit) - 1;
+        c0 = __builtin_amdgcn_readlane(a, l);
+        n = __builtin_amdgcn_readlane(b, l) - c0;
+        x = lo;
+        return true;
+    }
+    __shared__ int wsum[NW], found[3];
+    const int per = (p.seqs + 64 * NW - 1) / (64 * NW);
+    const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
     int sum = 0, a = s0 < s1 ? at(s0) : 0;
     for (int s = s0; s < s1; s++) {
         const int b = at(s + 1);
         sum += tiles(a, b);
         a = b;
     }
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(incl, o);
-        if (lane >= o) incl += v;
-    }
+    const int incl = wave_prefix(sum);
     if (lane == 63) wsum[wave] = incl;
     __syncthreads();
     int total = 0, before = 0;
@@ -122,17 +208,23 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
     return true;
 }
 
+// s_waitcnt lgkmcnt(0) that leaves the other counters alone, and keeps memory
+// accesses on their sides.
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // `odd`: 2 D + 1 words: per dim the first keys with values that are not finite
 // (tame, below), and whether there are any.
-template <class E, int D, int NQB, int KB, int NW>
+template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT>
 __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, int* odd, int c0, int n, int x, int kvh) {
-    using S = PackedTile<D, NQB, KB, NW>;
+    using S = PackedTile<D, NQB, KB, NW, NST, SPLIT>;
     constexpr int NG = S::NG, BK = S::BK;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lq = lane & 31,
               lh = lane >> 5;
     const int rows = n * p.G;                 // of the sequence
     const int row0 = x * S::RW;               // first of this tile
-    const int wrow = row0 + 32 * NQB * wave;  // first of this wave
+    const int wrow = row0 + (SPLIT ? 0 : 32 * NQB * wave);  // first of this wave
     // Query and head in the group of row r; rows past the sequence stand for
     // its last one and are not written.
     auto split = [&](int r, int& qi, int& hh) {
@@ -149,7 +241,8 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     // group g0 of block j0 on, lane i bringing 16 bytes of row g + NG (i /
     // (D / 8)) (K: of the piece that belongs at its place).
     constexpr int CH = D / 8;  // 16-byte pieces per row
-    const int j0 = wave * S::PER / NG, g0 = wave * S::PER % NG;
+    const int j0 = SPLIT ? 0 : wave * S::PER / NG, g0 = SPLIT ? 0 : wave * S::PER % NG;
+    if (SPLIT) smem += wave * (NST * S::STAGE);  // the wave's own stages
     const int lb = lane / CH, lc = lane % CH;
     const uint32_t k_row2 = (uint32_t)p.k_row * 2, v_row2 = (uint32_t)p.v_row * 2;
     const uint32_t piece_k = 16 * (lc ^ (D == 128 ? lb & 1 : D == 64 ? (lb >> 1) & 1 : 0)), piece_v = 16 * lc;
@@ -179,7 +272,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         }
     };
 
-    request(0, 0);
+    if (!SPLIT || wave < ntiles) request(SPLIT ? wave * BK : 0, 0);
     for (int i = tid; i <= 2 * D; i += S::THREADS) odd[i] = i < 2 * D ? 0x7fffffff : 0;
     uint4 qf[NQB][D / 16];
     int qi[NQB];
@@ -333,47 +426,98 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         }
     };
 
-    // Two stages: step i requests tile i + 1 into the stage that the barrier
-    // before it freed, computes tile i, waits for its own requests, and the
-    // barrier publishes tile i + 1.
     __syncthreads();  // `odd` is set
-    wait_vm<0>();
-    tame(0, 0);
-    __syncthreads();
-    for (int it = 0, buf = 0; it < ntiles; it++, buf ^= 1) {
-        const int k0 = it * BK;
-        const bool more = it + 1 < ntiles;
-        if (more) request(k0 + BK, buf ^ 1);
-        if (k0 <= last) compute(buf, k0);
-        if (more) {
+    if constexpr (SPLIT) {
+        // The wave's tiles wave, wave + NW, .. ; no other wave reads its stages.
+        for (int it = wave, buf = 0; it < ntiles; it += NW) {
+            const int k0 = it * BK;
+            const bool more = it + NW < ntiles;
             wait_vm<0>();
-            tame(k0 + BK, buf ^ 1);
-            __syncthreads();
+            tame(k0, buf);
+            wave_sync();
+            if (NST == 2 && more) request(k0 + NW * BK, buf ^ 1);
+            if (k0 <= last) compute(buf, k0);
+            wait_lds();  // the stage is read before the next request writes it
+            if (NST == 1 && more) request(k0 + NW * BK, 0);
+            if (NST == 2) buf ^= 1;
+        }
+        smem -= wave * (NST * S::STAGE);
+    } else {
+        // Two stages: step i requests tile i + 1 into the stage that the barrier
+        // before it freed, computes tile i, waits for its own requests, and the
+        // barrier publishes tile i + 1.
+        wait_vm<0>();
+        tame(0, 0);
+        __syncthreads();
+        for (int it = 0, buf = 0; it < ntiles; it++, buf ^= 1) {
+            const int k0 = it * BK;
+            const bool more = it + 1 < ntiles;
+            if (more) request(k0 + BK, buf ^ 1);
+            if (k0 <= last) compute(buf, k0);
+            if (more) {
+                wait_vm<0>();
+                tame(k0 + BK, buf ^ 1);
+                __syncthreads();
+            }
         }
     }
 
-    // Rows out: the wave's 32 columns are 32 rows, a lane holding 4-dim pieces
-    // of one, so they go through LDS (64 dims a pass, f32: the one rounding
-    // comes after the gate) and leave as 16-byte pieces, 8 lanes per row.
+    // Rows out: a lane holds 4-dim pieces of one row, so 32 columns are 32 rows
+    // and go through LDS (64 dims a pass, f32: the one rounding comes after the
+    // gate), and leave as 16-byte pieces, 8 lanes per row. SPLIT: the waves'
+    // sums, brought to the same maximum, are added there, each wave finishing
+    // 8 of the 32 rows.
+    constexpr int RK = SPLIT ? 32 / (8 * NW) : 4;  // rows a lane writes of each 32
+    static_assert(!SPLIT || NW == 4, "8 rows a wave");
+    __shared__ float join[SPLIT ? NW : 1][2][32];
+    if constexpr (SPLIT) {
+        l[0] = add_xor32(l[0]);
+        if (lh == 0) {
+            join[wave][0][lq] = m[0];
+            join[wave][1][lq] = l[0];
+        }
+    }
     __syncthreads();  // every wave is past the last tile's stage
     float* ew = reinterpret_cast<float*>(smem) + wave * 32 * S::RR;
     const int er = lane >> 3, ec = lane & 7;
     const bool any_odd = odd[2 * D] != 0;
 #pragma unroll
     for (int qb = 0; qb < NQB; qb++) {
-        const float inv = 1.f / add_xor32(l[qb]);
-        size_t t[4];
-        int head[4], query[4];
-        bool ok[4];
+        const int r0 = SPLIT ? 8 * wave : 0;  // of the block's rows
+        size_t t[RK];
+        int head[RK], query[RK];
+        bool ok[RK];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int r = wrow + 32 * qb + er + 8 * k;
+        for (int k = 0; k < RK; k++) {
+            const int r = wrow + 32 * qb + r0 + er + 8 * k;
             int qq, hh;
             split(r, qq, hh);
             ok[k] = r < rows;
             t[k] = (size_t)(c0 + qq);
             query[k] = qq;
             head[k] = kvh * p.G + hh;
+        }
+        // every pass's gates, requested before the first pass
+        uint4 gr[D / 64][RK];
+        if (p.gate) {
+#pragma unroll
+            for (int ps = 0; ps < D / 64; ps++)
+#pragma unroll
+                for (int k = 0; k < RK; k++)
+                    gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head +
+                                                                64 * ps + 8 * ec);
+        }
+        float inv;
+        if constexpr (SPLIT) {
+            float top = join[0][0][lq], sum = 0.f;
+#pragma unroll
+            for (int w = 1; w < NW; w++) top = fmaxf(top, join[w][0][lq]);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < NW; w++) sum += join[w][1][lq] * __builtin_amdgcn_exp2f(join[w][0][lq] - base);
+            inv = __builtin_amdgcn_exp2f(m[0] - base) / sum;
+        } else {
+            inv = 1.f / add_xor32(l[qb]);
         }
 #pragma unroll
         for (int ps = 0; ps < D / 64; ps++) {
@@ -385,12 +529,20 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                     *reinterpret_cast<float4*>(ew + lq * S::RR + 32 * (db - 2 * ps) + 8 * g + 4 * lh) =
                         make_float4(y[4 * g] * inv, y[4 * g + 1] * inv, y[4 * g + 2] * inv, y[4 * g + 3] * inv);
                 }
-            wave_sync();
+            if (SPLIT) __syncthreads();
+            else wave_sync();
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float* src = ew + (er + 8 * k) * S::RR + 8 * ec;
-                const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-                float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            for (int k = 0; k < RK; k++) {
+                const float* src = (SPLIT ? reinterpret_cast<float*>(smem) : ew) + (r0 + er + 8 * k) * S::RR + 8 * ec;
+                float y[8];
+#pragma unroll
+                for (int w = 0; w < (SPLIT ? NW : 1); w++) {
+                    const float4 a = *reinterpret_cast<const float4*>(src + w * 32 * S::RR),
+                                 b = *reinterpret_cast<const float4*>(src + w * 32 * S::RR + 4);
+                    const float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = w == 0 ? z[i] : y[i] + z[i];
+                }
                 if (any_odd) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
@@ -399,8 +551,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                     }
                 }
                 if (p.gate) {
-                    const uint4 g = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head +
-                                                                    64 * ps + 8 * ec);
+                    const uint4 g = gr[ps][k];
                     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -412,7 +563,9 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                     *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + 64 * ps + 8 * ec) =
                         make_uint4(E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7]));
             }
-            wave_sync();  // the region is rewritten by the next pass
+            // the region is rewritten by the next pass
+            if (SPLIT) __syncthreads();
+            else wave_sync();
         }
     }
 }
@@ -420,15 +573,18 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
 // 1-D grid of at least (tiles of the batch) x Hkv workgroups, kv heads first:
 // workgroup ids go to the 8 XCDs in turn, so with 1, 2, 4 or a multiple of 8
 // kv heads an XCD reads the K and V of few heads through its L2.
-template <class E, int D, int NQB, int KB, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) packed_kernel(PackedParams p) {
-    using S = PackedTile<D, NQB, KB, NW>;
+template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT, int OCC>
+__global__ void __launch_bounds__(64 * NW, OCC) packed_kernel(PackedParams p) {
+    using S = PackedTile<D, NQB, KB, NW, NST, SPLIT>;
     __shared__ __align__(16) char smem[S::LDS];
     __shared__ int odd[2 * D + 1];
     const int kvh = blockIdx.x % p.Hkv;
     int c0, n, x;
     if (!find_packed_tile<S::RW, NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
-    packed_tile<E, D, NQB, KB, NW>(p, smem, odd, c0, n, x, kvh);
+    c0 = __builtin_amdgcn_readfirstlane(c0);  // scalars, for the requests' bases
+    n = __builtin_amdgcn_readfirstlane(n);
+    x = __builtin_amdgcn_readfirstlane(x);
+    packed_tile<E, D, NQB, KB, NW, NST, SPLIT>(p, smem, odd, c0, n, x, kvh);
 }
 
 }  // namespace pkv

@@ -7,22 +7,31 @@
 
 namespace {
 
-template <class E, int D, int NQB, int KB, int NW>
-int launch(const pkv::PackedParams& p, int64_t T, hipStream_t stream) {
-    using S = pkv::PackedTile<D, NQB, KB, NW>;
-    // each sequence that has rows rounds up once
-    const int64_t tiles = (T * p.G + S::RW - 1) / S::RW + std::min<int64_t>(p.seqs, T);
-    if (tiles * p.Hkv * S::THREADS >= (int64_t)1 << 32) return PKV_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((pkv::packed_kernel<E, D, NQB, KB, NW>), dim3((unsigned)(tiles * p.Hkv)), dim3(S::THREADS), 0, stream,
-                       p);
+// Tiles of RW rows that the batch can have: each sequence with rows rounds up once.
+int64_t tile_bound(const pkv::PackedParams& p, int rw) {
+    return ((int64_t)p.T * p.G + rw - 1) / rw + std::min(p.seqs, p.T);
+}
+
+template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT, int OCC>
+int launch(const pkv::PackedParams& p, hipStream_t stream) {
+    using S = pkv::PackedTile<D, NQB, KB, NW, NST, SPLIT>;
+    const int64_t grid = tile_bound(p, S::RW) * p.Hkv;
+    if (grid * S::THREADS >= (int64_t)1 << 32) return PKV_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((pkv::packed_kernel<E, D, NQB, KB, NW, NST, SPLIT, OCC>), dim3((unsigned)grid), dim3(S::THREADS), 0,
+                       stream, p);
     return launch_status();
 }
 
 template <class E>
-int by_dims(const pkv::PackedParams& p, int D, int64_t T, hipStream_t stream) {
-    if (D == 64) return launch<E, 64, 1, 2, 4>(p, T, stream);
-    if (D == 128) return launch<E, 128, 1, 2, 4>(p, T, stream);
-    return launch<E, 256, 1, 1, 4>(p, T, stream);
+int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
+    if (tile_bound(p, 128) * p.Hkv < 128) {
+        if (D == 64) return launch<E, 64, 1, 1, 4, 2, true, 1>(p, stream);
+        if (D == 128) return launch<E, 128, 1, 1, 4, 1, true, 2>(p, stream);
+        return launch<E, 256, 1, 1, 4, 1, true, 1>(p, stream);
+    }
+    if (D == 64) return launch<E, 64, 1, 1, 4, 2, false, 4>(p, stream);
+    if (D == 128) return launch<E, 128, 1, 1, 4, 2, false, 3>(p, stream);
+    return launch<E, 256, 1, 1, 4, 2, false, 2>(p, stream);
 }
 
 }  // namespace
@@ -57,6 +66,6 @@ extern "C" int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, con
     p.cu = cu;
     p.seqs = seqs, p.T = T, p.Hkv = Hkv, p.G = Hq / Hkv;
     p.scale2 = scale * pkv::LOG2E;
-    return dtype == PKV_BF16 ? by_dims<pkv::Bf16>(p, D, T, (hipStream_t)stream)
-                             : by_dims<pkv::Fp16>(p, D, T, (hipStream_t)stream);
+    return dtype == PKV_BF16 ? by_dims<pkv::Bf16>(p, D, (hipStream_t)stream)
+                             : by_dims<pkv::Fp16>(p, D, (hipStream_t)stream);
 }

@@ -19,9 +19,9 @@ if not os.path.exists(LIB_PATH):
 # that already-loaded runtime, so device pointers and streams from torch are
 # valid in libpkv. Without torch the system ROCm runtime is used.
 try:
-    import torch  # noqa: F401
+    import torch
 except ImportError:
-    pass
+    torch = None
 _lib = ctypes.CDLL(LIB_PATH)
 
 OK = 0
@@ -348,7 +348,8 @@ def attn_prefill_workspace(T, Hq, Hkv, seqs):
 # Calls that take whole tensors (shapes, strides and types from them). A tensor
 # of another shape or type than the call's, on the CPU, or on another device
 # than the others, raises PkvError(ERR_INVALID) before anything is launched;
-# the launch is on the tensors' device, whichever is current.
+# the launch is on the tensors' device, whichever is current. (The checks are
+# written for their cost: a step's small calls are as long as their host time.)
 
 BF16, FP16 = 0, 1
 
@@ -359,55 +360,60 @@ def _refuse(what, why):
     raise e
 
 
-def _run(what, fn, tensors, stream, *args):
-    """fn(*args, stream) on the device that holds `tensors` (None: absent)."""
-    import torch
-    dev = -1
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        d = t.get_device()
-        if d < 0:
-            _refuse(what, f"{name} is not on a GPU")
-        if dev >= 0 and d != dev:
-            _refuse(what, f"{name} is on another device")
-        dev = d
+def _launch(what, fn, dev, stream, *args):
+    """fn(*args, stream) on device `dev`, stream None: torch's current one there."""
+    if dev < 0:
+        _refuse(what, "the tensors are not on a GPU")
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(dev)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
     if dev == torch.cuda.current_device():
-        _check(fn(*args, _stream(stream)), what)
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            _check(fn(*args, _stream(stream)), what)
+            status = fn(*args, stream)
+    if status != OK:
+        raise PkvError(status, what)
 
 
-def _ints(what, **arrays):
-    """int32 arrays without gaps; name=(tensor, numel) or (tensor, None)."""
-    import torch
-    for name, (t, n) in arrays.items():
-        if t.dtype is not torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
-            _refuse(what, f"{name} is not a contiguous int32 array" + ("" if n is None else f" of {n}"))
+def _words(what, dev, dtype, *arrays):
+    """The pointers of arrays (name, tensor, numel; None: any) of 32-bit words without gaps on device `dev`; None stays."""
+    out = []
+    for name, t, n in arrays:
+        if t is None:
+            out.append(None)
+            continue
+        if t.dtype is not dtype or (n is not None and t.numel() != n) or not t.is_contiguous():
+            _refuse(what, f"{name} is not a contiguous {dtype} array" + ("" if n is None else f" of {n}"))
+        if t.get_device() != dev:
+            _refuse(what, f"{name} is on another device")
+        out.append(t.data_ptr())
+    return out
 
 
-def _rows(what, T, H, D, dtype, **rows):
-    """[T, H, D] views of dtype (H None: any) whose last dim has no gaps."""
-    for name, t in rows.items():
-        s = t.shape
-        if t.dtype is not dtype or len(s) != 3 or s[0] != T or s[2] != D or (H is not None and s[1] != H) or (
-                D > 1 and t.stride(2) != 1):
-            _refuse(what, f"{name} is not [{T}, {'heads' if H is None else H}, {D}] rows of {dtype}, the last dim without gaps")
+def _rows(what, dev, dtype, T, H, D, name, t):
+    """Pointer, row and head stride of [T, H, D] rows whose last dim has no gaps (a stride that nobody steps by is given
+    as a dense one)."""
+    if t.dtype is not dtype or t.dim() != 3:
+        _refuse(what, f"{name} is not [{T}, {H}, {D}] rows of {dtype}")
+    n, h, d = t.shape
+    row, head, one = t.stride()
+    if n != T or h != H or d != D or one != 1:
+        _refuse(what, f"{name} is not [{T}, {H}, {D}] rows of {dtype}, the last dim without gaps")
+    if t.get_device() != dev:
+        _refuse(what, f"{name} is on another device")
+    return t.data_ptr(), row if T > 1 else H * D, head if H > 1 else D
 
 
-def _row_args(t):
-    """Pointer, row and head stride; a stride nobody steps by is given as one head's width."""
-    T, H, D = t.shape
-    return t.data_ptr(), t.stride(0) if T > 1 else H * D, t.stride(1) if H > 1 else D
-
-
-def _dtype(what, t):
-    import torch
-    if t.dtype is torch.bfloat16:
-        return BF16
-    if t.dtype is torch.float16:
-        return FP16
+def _row_type(what, q, k):
+    if q.dim() != 3 or k.dim() != 3:
+        _refuse(what, "q and k are not [T, heads, D]")
+    dtype = q.dtype
+    if dtype is torch.bfloat16:
+        return dtype, BF16
+    if dtype is torch.float16:
+        return dtype, FP16
     raise PkvError(ERR_UNSUPPORTED, what)
 
 
@@ -419,24 +425,18 @@ def plan_step(len, held, ntok, block_table, block_size, num_blocks, pos, slot_ma
     what = "pkv_plan_step"
     if block_table.dim() != 2:
         _refuse(what, "block_table is not [rows, max_blocks]")
-    n, T = block_table.shape[0], pos.numel()
-    _ints(what, len=(len, n), held=(held, n), ntok=(ntok, n), block_table=(block_table, None), pos=(pos, T),
-          slot_map=(slot_map, T), tok_seq=(tok_seq, T), cu=(cu, n + 1), limits=(limits, n), len_out=(len_out, n),
-          held_out=(held_out, n), status=(status, n))
-    if free_list is not None:
-        if free_list.numel() < num_blocks:
-            _refuse(what, "free_list holds fewer ids than the pool has pages")
-        _ints(what, free_list=(free_list, None))
-    for name, t in (("free_count", free_count), ("free_count_out", free_count_out)):
-        if t is not None:
-            _ints(what, **{name: (t, 1)})
-    _run(what, _lib.pkv_plan_step, dict(len=len, held=held, ntok=ntok, block_table=block_table, pos=pos, slot_map=slot_map,
-                                        tok_seq=tok_seq, cu=cu, limits=limits, len_out=len_out, held_out=held_out,
-                                        status=status, free_list=free_list, free_count=free_count,
-                                        free_count_out=free_count_out), stream,
-         _ptr(len), _ptr(held), _ptr(ntok), n, _ptr(block_table), block_table.shape[1], block_size, num_blocks,
-         _ptr(free_list), _ptr(free_count), T, _ptr(pos), _ptr(slot_map), _ptr(tok_seq), _ptr(cu), _ptr(limits),
-         _ptr(len_out), _ptr(held_out), _ptr(free_count_out), _ptr(status))
+    n, width = block_table.shape
+    T, dev = pos.numel(), pos.get_device()
+    if free_list is not None and free_list.numel() < num_blocks:
+        _refuse(what, "free_list holds fewer ids than the pool has pages")
+    (len, held, ntok, table, free_list, count, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out,
+     status) = _words(what, dev, torch.int32, ("len", len, n), ("held", held, n), ("ntok", ntok, n),
+                      ("block_table", block_table, None), ("free_list", free_list, None), ("free_count", free_count, 1),
+                      ("pos", pos, T), ("slot_map", slot_map, T), ("tok_seq", tok_seq, T), ("cu", cu, n + 1),
+                      ("limits", limits, n), ("len_out", len_out, n), ("held_out", held_out, n),
+                      ("free_count_out", free_count_out, 1), ("status", status, n))
+    _launch(what, _lib.pkv_plan_step, dev, stream, len, held, ntok, n, table, width, block_size, num_blocks, free_list,
+            count, T, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out, status)
 
 
 def plan_truncate(new_len, len, held, block_table, block_size, num_blocks, free_list, free_count, stream=None):
@@ -444,83 +444,72 @@ def plan_truncate(new_len, len, held, block_table, block_size, num_blocks, free_
     what = "pkv_plan_truncate"
     if block_table.dim() != 2:
         _refuse(what, "block_table is not [rows, max_blocks]")
-    n = block_table.shape[0]
-    _ints(what, new_len=(new_len, n), len=(len, n), held=(held, n), block_table=(block_table, None),
-          free_list=(free_list, None), free_count=(free_count, 1))
+    n, width = block_table.shape
+    dev = len.get_device()
     if free_list.numel() < num_blocks:
         _refuse(what, "free_list holds fewer ids than the pool has pages")
-    _run(what, _lib.pkv_plan_truncate, dict(new_len=new_len, len=len, held=held, block_table=block_table,
-                                            free_list=free_list, free_count=free_count), stream,
-         _ptr(new_len), _ptr(len), _ptr(held), n, _ptr(block_table), block_table.shape[1], block_size, num_blocks,
-         _ptr(free_list), _ptr(free_count))
+    new_len, len, held, table, free_list, count = _words(
+        what, dev, torch.int32, ("new_len", new_len, n), ("len", len, n), ("held", held, n),
+        ("block_table", block_table, None), ("free_list", free_list, None), ("free_count", free_count, 1))
+    _launch(what, _lib.pkv_plan_truncate, dev, stream, new_len, len, held, n, table, width, block_size, num_blocks,
+            free_list, count)
 
 
 def rope_spans(span_cu, spans, base, stream=None):
     """The position at which each media span of each request starts (see include/pkv.h): spans [n, 5] int32 rows
     (start, t, h, w, step), span_cu [requests + 1], base [n]."""
     what = "pkv_rope_spans"
-    n = spans.shape[0]
-    _ints(what, span_cu=(span_cu, None), spans=(spans, 5 * n), base=(base, n))
-    if span_cu.numel() < 1:
+    n, dev, req = spans.shape[0], spans.get_device(), span_cu.numel() - 1
+    if req < 0:
         _refuse(what, "span_cu is empty")
-    _run(what, _lib.pkv_rope_spans, dict(span_cu=span_cu, spans=spans, base=base), stream,
-         _ptr(span_cu), _ptr(spans), span_cu.numel() - 1, n, _ptr(base))
+    cu, spans, base = _words(what, dev, torch.int32, ("span_cu", span_cu, None), ("spans", spans, 5 * n), ("base", base, n))
+    _launch(what, _lib.pkv_rope_spans, dev, stream, cu, spans, req, n, base)
 
 
 def rope_positions(pos, tok_seq, span_cu, spans, base, rope, stream=None):
     """Time / height / width positions of a step's rows into rope [3, T] (or wider rows: rope[:, :T] is written)."""
     what = "pkv_rope_positions"
-    T, n = pos.numel(), spans.shape[0]
-    _ints(what, pos=(pos, T), tok_seq=(tok_seq, T), span_cu=(span_cu, None), spans=(spans, 5 * n), base=(base, n),
-          rope=(rope, None))
-    if span_cu.numel() < 1 or rope.dim() != 2 or rope.shape[0] != 3 or rope.shape[1] < T:
+    T, n, dev, req = pos.numel(), spans.shape[0], pos.get_device(), span_cu.numel() - 1
+    if req < 0 or rope.dim() != 2 or rope.shape[0] != 3 or rope.shape[1] < T:
         _refuse(what, f"rope is not [3, {T} or more], or span_cu is empty")
-    _run(what, _lib.pkv_rope_positions, dict(pos=pos, tok_seq=tok_seq, span_cu=span_cu, spans=spans, base=base, rope=rope),
-         stream, _ptr(pos), _ptr(tok_seq), T, _ptr(span_cu), _ptr(spans), _ptr(base), span_cu.numel() - 1, n, _ptr(rope),
-         rope.shape[1])
+    stride = rope.shape[1]
+    pos, seq, cu, spans, base, rope = _words(
+        what, dev, torch.int32, ("pos", pos, T), ("tok_seq", tok_seq, T), ("span_cu", span_cu, None),
+        ("spans", spans, 5 * n), ("base", base, n), ("rope", rope, None))
+    _launch(what, _lib.pkv_rope_positions, dev, stream, pos, seq, T, cu, spans, base, req, n, rope, stride)
 
 
 def rope_rows(q, k, rope, axes, inv_freq, q_out, k_out, q_norm=None, k_norm=None, eps=1e-6, adjacent=False, stream=None):
     """Norm (with weights) and rotation of q [T, Hq, D] and k [T, Hkv, D] rows into q_out and k_out (which may be q and
     k): rope [3, >= T] int32, axes [rot / 2] int32, inv_freq [rot / 2] f32 (see include/pkv.h)."""
-    import torch
     what = "pkv_rope_rows"
-    if q.dim() != 3 or k.dim() != 3:
-        _refuse(what, "q and k are not [T, heads, D]")
+    dtype, code = _row_type(what, q, k)
     T, Hq, D = q.shape
-    Hkv, dtype, half = k.shape[1], _dtype(what, q), axes.numel()
-    _rows(what, T, Hq, D, q.dtype, q=q, q_out=q_out)
-    _rows(what, T, Hkv, D, q.dtype, k=k, k_out=k_out)
-    _ints(what, rope=(rope, None), axes=(axes, half))
+    Hkv, half, dev = k.shape[1], axes.numel(), q.get_device()
     if rope.dim() != 2 or rope.shape[0] != 3 or rope.shape[1] < T:
         _refuse(what, f"rope is not [3, {T} or more]")
-    for name, t, n in (("inv_freq", inv_freq, half), ("q_norm", q_norm, D), ("k_norm", k_norm, D)):
-        if t is not None and (t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous()):
-            _refuse(what, f"{name} is not a contiguous float32 array of {n}")
-    _run(what, _lib.pkv_rope_rows, dict(q=q, k=k, rope=rope, axes=axes, inv_freq=inv_freq, q_out=q_out, k_out=k_out,
-                                        q_norm=q_norm, k_norm=k_norm), stream,
-         *_row_args(q), *_row_args(k), *_row_args(q_out), *_row_args(k_out), Hq, Hkv, D, dtype, _ptr(q_norm), _ptr(k_norm),
-         eps, _ptr(rope), rope.shape[1], _ptr(axes), _ptr(inv_freq), 2 * half, int(adjacent), T)
+    pos, ax = _words(what, dev, torch.int32, ("rope", rope, None), ("axes", axes, half))
+    inv, qn, kn = _words(what, dev, torch.float32, ("inv_freq", inv_freq, half), ("q_norm", q_norm, D), ("k_norm", k_norm, D))
+    _launch(what, _lib.pkv_rope_rows, dev, stream, *_rows(what, dev, dtype, T, Hq, D, "q", q),
+            *_rows(what, dev, dtype, T, Hkv, D, "k", k), *_rows(what, dev, dtype, T, Hq, D, "q_out", q_out),
+            *_rows(what, dev, dtype, T, Hkv, D, "k_out", k_out), Hq, Hkv, D, code, qn, kn, eps, pos, rope.shape[1], ax, inv,
+            2 * half, adjacent, T)
 
 
 def attn_packed(q, k, v, cu, out, scale, gate=None, stream=None):
     """Causal attention over packed whole prompts, no cache (see include/pkv.h): q, out (and gate) [T, Hq, D], k and v
     [T, Hkv, D] of bfloat16 or float16, any row and head strides; cu [sequences + 1] int32."""
     what = "pkv_attn_packed"
-    if q.dim() != 3 or k.dim() != 3:
-        _refuse(what, "q and k are not [T, heads, D]")
+    dtype, code = _row_type(what, q, k)
     T, Hq, D = q.shape
-    Hkv, dtype = k.shape[1], _dtype(what, q)
-    _rows(what, T, Hq, D, q.dtype, q=q, out=out)
-    _rows(what, T, Hkv, D, q.dtype, k=k, v=v)
-    if gate is not None:
-        _rows(what, T, Hq, D, q.dtype, gate=gate)
-    _ints(what, cu=(cu, None))
-    if cu.numel() < 1:
+    Hkv, dev, seqs = k.shape[1], q.get_device(), cu.numel() - 1
+    if seqs < 0:
         _refuse(what, "cu is empty")
-    _run(what, _lib.pkv_attn_packed, dict(q=q, k=k, v=v, cu=cu, out=out, gate=gate), stream,
-         *_row_args(q), *_row_args(k), *_row_args(v), *((None, 0, 0) if gate is None else _row_args(gate)),
-         *_row_args(out), _ptr(cu), cu.numel() - 1, T, Hq, Hkv, D, dtype, scale)
+    (offsets,) = _words(what, dev, torch.int32, ("cu", cu, None))
+    _launch(what, _lib.pkv_attn_packed, dev, stream, *_rows(what, dev, dtype, T, Hq, D, "q", q),
+            *_rows(what, dev, dtype, T, Hkv, D, "k", k), *_rows(what, dev, dtype, T, Hkv, D, "v", v),
+            *((None, 0, 0) if gate is None else _rows(what, dev, dtype, T, Hq, D, "gate", gate)),
+            *_rows(what, dev, dtype, T, Hq, D, "out", out), offsets, seqs, T, Hq, Hkv, D, code, scale)
 
 
 class Pool:

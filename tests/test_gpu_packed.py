@@ -102,7 +102,9 @@ def test_any_group(dev, G):
 
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_long_prompts_and_many_sequences(dev, D):
-    for lens, Hq, Hkv in (([5000], 2, 1), ([1 + 7 * i % 50 for i in range(700)], 4, 2)):
+    for lens, Hq, Hkv in (([5000], 2, 1), ([1 + 7 * i % 50 for i in range(700)], 4, 2),
+                          ([1 + 37 * i % 211 for i in range(256)], 5, 1), ([1 + 37 * i % 211 for i in range(257)], 5, 1),
+                          ([500, 3, 0, 900, 0, 0, 1300, 65], 8, 2)):
         print("case", D, len(lens), flush=True)
         c = inputs(lens, Hq, Hkv, D, "bf16", D, dev)
         check(c, run(c), f"D {D}, {len(lens)} sequences")
@@ -128,25 +130,29 @@ def test_views_of_a_projection_row(dev):
     check(c, run(c), "broadcast kv heads")
 
 
+@pytest.mark.parametrize("more", [[], [129] * 60, [1] * 300 + [129] * 60])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_rows_outside_the_sequences(dev, D):
+def test_rows_outside_the_sequences(dev, D, more):
     """Rows before the first and behind the last sequence, NaN in them: neither read into others nor written."""
-    c = inputs([70, 0, 33], 4, 2, D, "bf16", 5, dev, gate=True, lead=9, tail=50)
-    inner = slice(9, 9 + 103)
+    c = inputs([70, 0, 33] + more, 4, 2, D, "bf16", 5, dev, gate=True, lead=9, tail=50)
+    n = 103 + sum(more)
+    inner = slice(9, 9 + n)
     clean = run(c)
-    for n in ("q", "k", "v", "gate"):
-        keep = c[n][inner].clone()
-        c[n].fill_(float("nan"))
-        c[n][inner] = keep
+    for x in ("q", "k", "v", "gate"):
+        keep = c[x][inner].clone()
+        c[x].fill_(float("nan"))
+        c[x][inner] = keep
     got = run(c)
     assert torch.equal(got[inner], clean[inner])
-    assert (got[:9] == 7).all() and (got[9 + 103:] == 7).all()
+    assert (got[:9] == 7).all() and (got[9 + n:] == 7).all()
 
 
+@pytest.mark.parametrize("more", [[], [129] * 40, [1] * 300 + [129] * 40])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_infinite_and_nan_values_reach_the_rows_that_attend_them(dev, D, dtype):
-    lens, Hq, Hkv = [150, 40], 6, 2
+def test_infinite_and_nan_values_reach_the_rows_that_attend_them(dev, D, dtype, more):
+    """Alone (few tiles), and in batches of many tiles and many sequences."""
+    lens, Hq, Hkv = [150, 40] + more, 6, 2
     c = inputs(lens, Hq, Hkv, D, dtype, 11, dev)
     clean = run(c)
     inf = float("inf")
@@ -183,20 +189,23 @@ def test_infinite_and_nan_values_reach_the_rows_that_attend_them(dev, D, dtype):
 
 
 def test_gates_at_their_ends(dev):
-    """Gates that close a row (down to the smallest results), open it, are infinite or NaN, and one on an infinite value."""
+    """Gates that close a row, open it, are infinite or NaN, and one on an infinite value. Below -87.3 the result is 0,
+    within 1.2e-38 of the value: the bound's smallest term is below that, so those two dims are held to it alone."""
     c = inputs([60], 4, 2, 64, "bf16", 12, dev, gate=True)
-    ends = torch.tensor([-87.0, -87.5, -88.5, -100.0, -30.0, 0.0, 20.0, 88.0, 3e38], device=dev).bfloat16()
+    ends = torch.tensor([-87.0, -86.5, -80.0, -60.0, -30.0, 0.0, 20.0, 88.0, 3e38], device=dev).bfloat16()
     c["gate"][:, :, :9] = ends
     plain = run(dict(c, gate=None))
     got = run(c)
     check(c, got, "gates")
     # (0.01 e^-87 is above 2^-133, the smallest number)
     assert (got[:, :, 0] != 0)[plain[:, :, 0].abs() > 0.01].all() and torch.equal(got[:, :, 8], plain[:, :, 8])
+    c["gate"][:, :, 3], c["gate"][:, :, 4] = -88.0, -1000.0
+    assert (run(c)[:, :, 3:5].abs() <= 1.2e-38 * plain.abs().max()).all()
     c["gate"][:, :, 0], c["gate"][:, :, 1], c["gate"][:, :, 2] = -float("inf"), float("inf"), float("nan")
-    c["v"][30, 0, 5] = float("inf")
+    c["v"][30, 0, 6] = float("inf")
     got = run(c)
     assert (got[:, :, 0] == 0).all() and torch.equal(got[:, :, 1], plain[:, :, 1]) and torch.isnan(got[:, :, 2]).all()
-    assert (got[30:, :2, 5] == float("inf")).all()
+    assert (got[30:, :2, 6] == float("inf")).all()
 
 
 def test_scores_of_minus_infinity_first(dev):
