@@ -34,21 +34,6 @@ int vec_mode(const void* a, const void* b, const void* c, const void* d, int64_t
     return 0;
 }
 
-// Compute units of the current device, cached per device.
-int device_cus() {
-    static std::mutex mu;
-    static int cus[64] = {0};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    std::lock_guard<std::mutex> g(mu);
-    if (cus[dev] == 0) {
-        int n = 0;
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-        cus[dev] = n;
-    }
-    return cus[dev];
-}
-
 int g_wg_per_cu = 1;
 int g_min_range = 32;
 // Events the next key-range launch of this thread records at its start and

@@ -38,14 +38,13 @@ struct PackedParams {
     float scale2;  // scale * log2(e)
 };
 
-// Shapes of a workgroup: D dims a head, NW waves of 32 NQB rows, tiles of KB
-// blocks of 32 keys, NST stages. SPLIT: the waves have the same 32 NQB rows and
-// take the key tiles in turn, each through stages of its own, and the waves'
-// sums are joined at the end.
-template <int D, int NQB, int KB, int NW, int NST = 2, bool SPLIT = false>
+// Shapes of a workgroup for heads of D dims: RG x KS waves, RG of them with 32
+// rows each, KS times over: key group g of KS takes the 32-key tiles g, g + KS,
+// .. through NST stages of its own, and the groups' sums are joined at the end.
+template <int D, int RG, int KS, int NST>
 struct PackedTile {
-    static constexpr int RW = 32 * NQB * (SPLIT ? 1 : NW), BK = 32 * KB, THREADS = 64 * NW;
-    // A 32-row block of K or V in LDS: NG groups of 1,024 bytes, one LDS DMA
+    static constexpr int RW = 32 * RG, NW = RG * KS, THREADS = 64 * NW;
+    // A tile of K or V in LDS: NG groups of 1,024 bytes, one LDS DMA
     // instruction each; row r lies in group r % NG at (r / NG) 2 D bytes.
     // K groups are 1,056 bytes apart (1,040 at 256 dims) and rows with bit 3
     // set have their 16-byte pieces swapped in pairs, so the 16 rows that a
@@ -54,16 +53,14 @@ struct PackedTile {
     // a half-wave's transposing read lie on distinct banks.
     static constexpr int NG = D / 16;
     static constexpr int KG = D == 256 ? 1040 : 1056, VG = 1088;
-    static constexpr int KBLK = NG * KG, VBLK = NG * VG;
-    static constexpr int STAGE = KB * (KBLK + VBLK);
-    static constexpr int PER = KB * NG / (SPLIT ? 1 : NW);  // groups of K (and of V) that a wave requests per tile
-    static constexpr int RR = 68;             // staged output row, floats of 64 dims
+    static constexpr int STAGE = NG * (KG + VG);
+    static constexpr int PER = NG / RG;  // groups of K (and of V) that a wave requests per tile
+    static constexpr int RR = 68;        // staged output row, floats of 64 dims
     static constexpr int EPI = NW * 32 * RR * 4;
-    static constexpr int STAGES = NST * (SPLIT ? NW : 1) * STAGE;
+    static constexpr int STAGES = NST * KS * STAGE;
     static constexpr int LDS = STAGES > EPI ? STAGES : EPI;
-    static_assert(KB * NG % NW == 0 && NG % PER == 0, "a wave's groups lie in one block");
-    static_assert(NST == 2 || (SPLIT && NST == 1), "two stages, or one per wave");
-    static_assert(!SPLIT || NQB == 1, "32 rows");
+    static_assert(NG % RG == 0 && 4 % KS == 0, "whole groups a wave, whole 8-row pieces a key group");
+    static_assert(NST == 2 || (RG == 1 && NST == 1), "two stages, or one where a wave has it for itself");
     static __device__ __forceinline__ constexpr int swap(int r) { return D == 256 ? 0 : (r >> 3) & 1; }
 };
 
@@ -216,15 +213,16 @@ __device__ __forceinline__ void wait_lds() {
 
 // `odd`: 2 D + 1 words: per dim the first keys with values that are not finite
 // (tame, below), and whether there are any.
-template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT>
+template <class E, int D, int RG, int KS, int NST>
 __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, int* odd, int c0, int n, int x, int kvh) {
-    using S = PackedTile<D, NQB, KB, NW, NST, SPLIT>;
-    constexpr int NG = S::NG, BK = S::BK;
+    using S = PackedTile<D, RG, KS, NST>;
+    constexpr int NG = S::NG, BK = 32, NW = S::NW;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lq = lane & 31,
               lh = lane >> 5;
-    const int rows = n * p.G;                 // of the sequence
-    const int row0 = x * S::RW;               // first of this tile
-    const int wrow = row0 + (SPLIT ? 0 : 32 * NQB * wave);  // first of this wave
+    const int rg = wave % RG, kg = wave / RG;  // row group, key group
+    const int rows = n * p.G;                  // of the sequence
+    const int row0 = x * S::RW;                // first of this tile
+    const int wrow = row0 + 32 * rg;           // first of this wave
     // Query and head in the group of row r; rows past the sequence stand for
     // its last one and are not written.
     auto split = [&](int r, int& qi, int& hh) {
@@ -234,33 +232,34 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     };
     const int L = (min(row0 + S::RW, rows) - 1) / p.G + 1;  // keys of this tile
     const int ntiles = (L + BK - 1) / BK;
-    // the wave's last query (below the first key: no rows)
-    const int last = wrow < rows ? (min(wrow + 32 * NQB, rows) - 1) / p.G : -1;
+    const int first_q = row0 / p.G;                          // of the tile
+    const int wfirst = min(wrow, rows - 1) / p.G;            // of the wave
+    const int last = wrow < rows ? (min(wrow + 32, rows) - 1) / p.G : -1;  // the wave's last (no rows: none)
 
-    // Requests of K and V rows, straight to LDS: the wave's PER groups from
-    // group g0 of block j0 on, lane i bringing 16 bytes of row g + NG (i /
-    // (D / 8)) (K: of the piece that belongs at its place).
+    // Requests of K and V rows, straight to LDS: the wave's PER groups of its
+    // key group's tile, lane i bringing 16 bytes of row g + NG (i / (D / 8))
+    // (K: of the piece that belongs at its place).
     constexpr int CH = D / 8;  // 16-byte pieces per row
-    const int j0 = SPLIT ? 0 : wave * S::PER / NG, g0 = SPLIT ? 0 : wave * S::PER % NG;
-    if (SPLIT) smem += wave * (NST * S::STAGE);  // the wave's own stages
+    char* const stage = smem + kg * (NST * S::STAGE);
+    const int g0 = rg * S::PER;
     const int lb = lane / CH, lc = lane % CH;
     const uint32_t k_row2 = (uint32_t)p.k_row * 2, v_row2 = (uint32_t)p.v_row * 2;
     const uint32_t piece_k = 16 * (lc ^ (D == 128 ? lb & 1 : D == 64 ? (lb >> 1) & 1 : 0)), piece_v = 16 * lc;
     const uint32_t off_k = (uint32_t)(NG * lb) * k_row2 + piece_k, off_v = (uint32_t)(NG * lb) * v_row2 + piece_v;
     const char* kb = reinterpret_cast<const char*>(p.k + c0 * p.k_row + kvh * p.k_head);
     const char* vb = reinterpret_cast<const char*>(p.v + c0 * p.v_row + kvh * p.v_head);
-    const uint32_t lds0 = lds_addr(smem);
+    const uint32_t lds0 = lds_addr(stage);
     auto request = [&](int k0, int buf) __attribute__((always_inline)) {
-        const uint32_t lk = lds0 + buf * S::STAGE + j0 * S::KBLK + g0 * S::KG;
-        const uint32_t lv = lds0 + buf * S::STAGE + KB * S::KBLK + j0 * S::VBLK + g0 * S::VG;
-        const int r0 = k0 + 32 * j0 + g0;
+        const uint32_t lk = lds0 + buf * S::STAGE + g0 * S::KG;
+        const uint32_t lv = lds0 + buf * S::STAGE + NG * S::KG + g0 * S::VG;
+        const int r0 = k0 + g0;
         if (k0 + BK <= L) {
-            const char* kg = kb + (size_t)r0 * k_row2;
-            const char* vg = vb + (size_t)r0 * v_row2;
+            const char* ks = kb + (size_t)r0 * k_row2;
+            const char* vs = vb + (size_t)r0 * v_row2;
 #pragma unroll
-            for (int i = 0; i < S::PER; i++) dma16_s(kg + (size_t)i * k_row2, off_k, lk + i * S::KG);
+            for (int i = 0; i < S::PER; i++) dma16_s(ks + (size_t)i * k_row2, off_k, lk + i * S::KG);
 #pragma unroll
-            for (int i = 0; i < S::PER; i++) dma16_s(vg + (size_t)i * v_row2, off_v, lv + i * S::VG);
+            for (int i = 0; i < S::PER; i++) dma16_s(vs + (size_t)i * v_row2, off_v, lv + i * S::VG);
         } else {
             // the last tile: rows past the keys stand for the last key
 #pragma unroll
@@ -272,135 +271,101 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         }
     };
 
-    if (!SPLIT || wave < ntiles) request(SPLIT ? wave * BK : 0, 0);
+    if (kg < ntiles) request(kg * BK, 0);
     for (int i = tid; i <= 2 * D; i += S::THREADS) odd[i] = i < 2 * D ? 0x7fffffff : 0;
-    uint4 qf[NQB][D / 16];
-    int qi[NQB];
-#pragma unroll
-    for (int qb = 0; qb < NQB; qb++) {
+    uint4 qf[D / 16];
+    int qi;
+    {
         int hh;
-        split(wrow + 32 * qb + lq, qi[qb], hh);
-        const uint16_t* src = p.q + (size_t)(c0 + qi[qb]) * p.q_row + (size_t)(kvh * p.G + hh) * p.q_head + 8 * lh;
+        split(wrow + lq, qi, hh);
+        const uint16_t* src = p.q + (size_t)(c0 + qi) * p.q_row + (size_t)(kvh * p.G + hh) * p.q_head + 8 * lh;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) qf[qb][kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
+        for (int kk = 0; kk < D / 16; kk++) qf[kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
     }
-    f32x16 o[NQB][D / 32];
-    float m[NQB], l[NQB];  // running maximum (log2 units, may lag, below); the lane's own part of the sum
+    f32x16 o[D / 32];
+    float m = -INFINITY, l = 0.f;  // running maximum (log2 units, may lag, below); the lane's own part of the sum
 #pragma unroll
-    for (int qb = 0; qb < NQB; qb++) {
-        m[qb] = -INFINITY;
-        l[qb] = 0.f;
+    for (int db = 0; db < D / 32; db++)
 #pragma unroll
-        for (int db = 0; db < D / 32; db++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[qb][db][r] = 0.f;
-    }
+        for (int r = 0; r < 16; r++) o[db][r] = 0.f;
 
-    // Lane addresses in a block of K and V (bytes).
+    // Lane addresses in a tile of K and V (bytes).
     const int k_at = (lq % NG) * S::KG + lq / NG * (2 * D) + 16 * (lh ^ S::swap(lq));
     const int tr_r = 4 * lh + ((lane & 15) >> 2);  // + 16 kk + 8 h: row of the transposing read
-    const int v_at = tr_r % NG * S::VG + tr_r / NG * (2 * D) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-    // row + 8 h + 16 kk of the block, from v_at
+    const int v_at = NG * S::KG + tr_r % NG * S::VG + tr_r / NG * (2 * D) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    // row + 8 h + 16 kk of the tile, from v_at
     auto v_step = [](int kk, int h) constexpr { return D == 256 ? h * 8 * S::VG + kk * 2 * D : (16 * kk + 8 * h) / NG * 2 * D; };
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    auto v_frag = [&](const char* V, int kk, int db) __attribute__((always_inline)) {
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 0) + 64 * db));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 1) + 64 * db));
-        return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
 
     auto compute = [&](int buf, int k0) __attribute__((always_inline)) {
-        const char* K = smem + buf * S::STAGE + k_at;
-        const char* V = smem + buf * S::STAGE + KB * S::KBLK + v_at;
-        f32x16 st[KB][NQB];
+        const char* K = stage + buf * S::STAGE + k_at;
+        const char* V = stage + buf * S::STAGE + v_at;
+        f32x16 st;
 #pragma unroll
-        for (int j = 0; j < KB; j++) {
+        for (int r = 0; r < 16; r++) st[r] = 0.f;
 #pragma unroll
-            for (int qb = 0; qb < NQB; qb++)
+        for (int kk = 0; kk < D / 16; kk++) st = E::mfma(*reinterpret_cast<const uint4*>(K + 32 * kk), qf[kk], st);
+        if (k0 + BK - 1 > wfirst) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) st[j][qb][r] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) {
-                const uint4 a = *reinterpret_cast<const uint4*>(K + j * S::KBLK + 32 * kk);
-#pragma unroll
-                for (int qb = 0; qb < NQB; qb++) st[j][qb] = E::mfma(a, qf[qb][kk], st[j][qb]);
-            }
+            for (int r = 0; r < 16; r++)
+                if (k0 + 8 * (r >> 2) + 4 * lh + (r & 3) > qi) st[r] = -INFINITY;
         }
-        uint4 pb[KB][NQB][2];
+        float mx = st[0];
 #pragma unroll
-        for (int qb = 0; qb < NQB; qb++) {
-            const int qfirst = min(wrow + 32 * qb, rows - 1) / p.G;
-            if (k0 + BK - 1 > qfirst) {
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[r]);
+        mx = max_xor32(mx) * p.scale2;
+        // The maximum may lag behind by up to 8: weights up to 2^8, all of a
+        // row relative to the same power, so no digit is lost, and the
+        // rescaling of O is skipped in almost every tile.
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= corr;
 #pragma unroll
-                for (int j = 0; j < KB; j++)
+            for (int db = 0; db < D / 32; db++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (k0 + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3) > qi[qb]) st[j][qb][r] = -INFINITY;
+                for (int r = 0; r < 16; r++) o[db][r] *= corr;
+        }
+        // scores of -inf so far: their weight is 0, not NaN
+        const float base = m == -INFINITY ? 0.f : m;
+        // P is rounded to the type of the rows, as the matrix units take it;
+        // the sum is of the rounded weights, so they still add up to 1.
+        uint4 pb[2];
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float s0 = st[8 * kk + 2 * i], s1 = st[8 * kk + 2 * i + 1];
+                w[i] = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.scale2, -base)),
+                               __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.scale2, -base)));
+                l = E::dot(w[i], E::ONE, l);
             }
-            float mx = st[0][qb][0];
-#pragma unroll
-            for (int j = 0; j < KB; j++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[j][qb][r]);
-            mx = max_xor32(mx) * p.scale2;
-            // The maximum may lag behind by up to 8: weights up to 2^8, all of
-            // a row relative to the same power, so no digit is lost, and the
-            // rescaling of O is skipped in almost every tile.
-            if (__any(mx > m[qb] + 8.f)) {
-                const float mn = fmaxf(m[qb], mx);
-                const float corr = __builtin_amdgcn_exp2f(m[qb] - (mn == -INFINITY ? 0.f : mn));
-                m[qb] = mn;
-                l[qb] *= corr;
-#pragma unroll
-                for (int db = 0; db < D / 32; db++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[qb][db][r] *= corr;
-            }
-            // scores of -inf so far: their weight is 0, not NaN
-            const float base = m[qb] == -INFINITY ? 0.f : m[qb];
-            // P is rounded to the type of the rows, as the matrix units take
-            // it; the sum is of the rounded weights, so they still add up to 1.
-#pragma unroll
-            for (int j = 0; j < KB; j++)
-#pragma unroll
-                for (int kk = 0; kk < 2; kk++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float s0 = st[j][qb][8 * kk + 2 * i], s1 = st[j][qb][8 * kk + 2 * i + 1];
-                        w[i] = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.scale2, -base)),
-                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.scale2, -base)));
-                        l[qb] = E::dot(w[i], E::ONE, l[qb]);
-                    }
-                    pb[j][qb][kk] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+            pb[kk] = make_uint4(w[0], w[1], w[2], w[3]);
         }
 #pragma unroll
-        for (int j = 0; j < KB; j++)
+        for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-                for (int db = 0; db < D / 32; db++) {
-                    const uint4 a = v_frag(V + j * S::VBLK, kk, db);
-#pragma unroll
-                    for (int qb = 0; qb < NQB; qb++) o[qb][db] = E::mfma(a, pb[j][qb][kk], o[qb][db]);
-                }
+            for (int db = 0; db < D / 32; db++) {
+                const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 0) + 64 * db));
+                const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + v_step(kk, 1) + 64 * db));
+                o[db] = E::mfma(__builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)), pb[kk], o[db]);
+            }
     };
 
     // A weight of 0 times an infinite or NaN value is NaN, so a value must not
     // meet the weights of rows that do not attend its key. Only tiles with
-    // keys behind the tile's first query can hold such a pair: there the wave
-    // looks through the values that it brought, takes out what is not finite,
-    // and notes for its dim the first key with (+inf or NaN) and with (-inf or
-    // NaN). A row attends a key if and only if the key is not behind it, so
-    // those two say what the finished rows get.
-    const int first_q = row0 / p.G;
+    // keys behind the workgroup's first query can hold such a pair: there the
+    // wave looks through the values that it brought, takes out what is not
+    // finite, and notes for its dim the first key with (+inf or NaN) and with
+    // (-inf or NaN). A row attends a key if and only if the key is not behind
+    // it, so those two say what the finished rows get.
     auto tame = [&](int k0, int buf) __attribute__((always_inline)) {
         if (k0 + BK - 1 <= first_q) return;
 #pragma unroll
         for (int i = 0; i < S::PER; i++) {
-            uint4* at = reinterpret_cast<uint4*>(smem + buf * S::STAGE + KB * S::KBLK + j0 * S::VBLK + (g0 + i) * S::VG +
-                                                 16 * lane);
+            uint4* at = reinterpret_cast<uint4*>(stage + buf * S::STAGE + NG * S::KG + (g0 + i) * S::VG + 16 * lane);
             const uint4 x = *at;
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             bool bad = false;
@@ -410,7 +375,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                 bad |= (u & 0xffffu) == 0 || (u >> 16) == 0;
             }
             if (bad) {
-                const int key = k0 + 32 * j0 + g0 + i + NG * lb;
+                const int key = k0 + g0 + i + NG * lb;
 #pragma unroll 1
                 for (int e = 0; e < 8; e++) {
                     const uint32_t y = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
@@ -427,36 +392,34 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     };
 
     __syncthreads();  // `odd` is set
-    if constexpr (SPLIT) {
-        // The wave's tiles wave, wave + NW, .. ; no other wave reads its stages.
-        for (int it = wave, buf = 0; it < ntiles; it += NW) {
+    if constexpr (RG == 1) {
+        // The wave has its tiles for itself: no barriers.
+        for (int it = kg, buf = 0; it < ntiles; it += KS) {
             const int k0 = it * BK;
-            const bool more = it + NW < ntiles;
+            const bool more = it + KS < ntiles;
             wait_vm<0>();
             tame(k0, buf);
             wave_sync();
-            if (NST == 2 && more) request(k0 + NW * BK, buf ^ 1);
+            if (NST == 2 && more) request(k0 + KS * BK, buf ^ 1);
             if (k0 <= last) compute(buf, k0);
             wait_lds();  // the stage is read before the next request writes it
-            if (NST == 1 && more) request(k0 + NW * BK, 0);
+            if (NST == 1 && more) request(k0 + KS * BK, 0);
             if (NST == 2) buf ^= 1;
         }
-        smem -= wave * (NST * S::STAGE);
     } else {
-        // Two stages: step i requests tile i + 1 into the stage that the barrier
-        // before it freed, computes tile i, waits for its own requests, and the
-        // barrier publishes tile i + 1.
+        // Two stages: a step requests its key group's next tile into the stage
+        // that the barrier before it freed, computes its tile, waits for its own
+        // requests, and the barrier publishes the next tile.
         wait_vm<0>();
-        tame(0, 0);
+        if (kg < ntiles) tame(kg * BK, 0);
         __syncthreads();
-        for (int it = 0, buf = 0; it < ntiles; it++, buf ^= 1) {
-            const int k0 = it * BK;
-            const bool more = it + 1 < ntiles;
-            if (more) request(k0 + BK, buf ^ 1);
+        for (int it = 0, buf = 0; it < ntiles; it += KS, buf ^= 1) {
+            const int k0 = (it + kg) * BK, k1 = k0 + KS * BK;
+            if (k1 < L) request(k1, buf ^ 1);
             if (k0 <= last) compute(buf, k0);
-            if (more) {
+            if (it + KS < ntiles) {
                 wait_vm<0>();
-                tame(k0 + BK, buf ^ 1);
+                if (k1 < L) tame(k1, buf ^ 1);
                 __syncthreads();
             }
         }
@@ -464,127 +427,122 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
 
     // Rows out: a lane holds 4-dim pieces of one row, so 32 columns are 32 rows
     // and go through LDS (64 dims a pass, f32: the one rounding comes after the
-    // gate), and leave as 16-byte pieces, 8 lanes per row. SPLIT: the waves'
-    // sums, brought to the same maximum, are added there, each wave finishing
-    // 8 of the 32 rows.
-    constexpr int RK = SPLIT ? 32 / (8 * NW) : 4;  // rows a lane writes of each 32
-    static_assert(!SPLIT || NW == 4, "8 rows a wave");
-    __shared__ float join[SPLIT ? NW : 1][2][32];
-    if constexpr (SPLIT) {
-        l[0] = add_xor32(l[0]);
+    // gate), and leave as 16-byte pieces, 8 lanes per row. With several key
+    // groups their sums, brought to the same maximum, are added there, each
+    // group's wave finishing its part of the 32 rows.
+    constexpr int RK = 4 / KS;  // rows a lane writes
+    __shared__ float join[KS > 1 ? NW : 1][2][32];
+    if constexpr (KS > 1) {
+        l = add_xor32(l);
         if (lh == 0) {
-            join[wave][0][lq] = m[0];
-            join[wave][1][lq] = l[0];
+            join[wave][0][lq] = m;
+            join[wave][1][lq] = l;
         }
     }
     __syncthreads();  // every wave is past the last tile's stage
-    float* ew = reinterpret_cast<float*>(smem) + wave * 32 * S::RR;
+    float* const out_stage = reinterpret_cast<float*>(smem) + rg * 32 * S::RR;  // key group g's: + g RG 32 RR
     const int er = lane >> 3, ec = lane & 7;
     const bool any_odd = odd[2 * D] != 0;
+    size_t t[RK];
+    int head[RK], query[RK];
+    bool ok[RK];
 #pragma unroll
-    for (int qb = 0; qb < NQB; qb++) {
-        const int r0 = SPLIT ? 8 * wave : 0;  // of the block's rows
-        size_t t[RK];
-        int head[RK], query[RK];
-        bool ok[RK];
+    for (int k = 0; k < RK; k++) {
+        const int r = wrow + 8 * RK * kg + er + 8 * k;
+        int hh;
+        split(r, query[k], hh);
+        ok[k] = r < rows;
+        t[k] = (size_t)(c0 + query[k]);
+        head[k] = kvh * p.G + hh;
+    }
+    // every pass's gates, requested before the first pass
+    uint4 gr[D / 64][RK];
+    if (p.gate) {
+#pragma unroll
+        for (int ps = 0; ps < D / 64; ps++)
+#pragma unroll
+            for (int k = 0; k < RK; k++)
+                gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head + 64 * ps +
+                                                            8 * ec);
+    }
+    float inv;
+    if constexpr (KS > 1) {
+        float top = m, sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < KS; g++) top = fmaxf(top, join[g * RG + rg][0][lq]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int g = 0; g < KS; g++) sum += join[g * RG + rg][1][lq] * __builtin_amdgcn_exp2f(join[g * RG + rg][0][lq] - base);
+        inv = __builtin_amdgcn_exp2f(m - base) / sum;
+    } else {
+        inv = 1.f / add_xor32(l);
+    }
+#pragma unroll
+    for (int ps = 0; ps < D / 64; ps++) {
+#pragma unroll
+        for (int db = 2 * ps; db < 2 * ps + 2; db++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const f32x16& y = o[db];
+                *reinterpret_cast<float4*>(out_stage + kg * (RG * 32 * S::RR) + lq * S::RR + 32 * (db - 2 * ps) + 8 * g +
+                                           4 * lh) =
+                    make_float4(y[4 * g] * inv, y[4 * g + 1] * inv, y[4 * g + 2] * inv, y[4 * g + 3] * inv);
+            }
+        if (KS > 1) __syncthreads();
+        else wave_sync();
 #pragma unroll
         for (int k = 0; k < RK; k++) {
-            const int r = wrow + 32 * qb + r0 + er + 8 * k;
-            int qq, hh;
-            split(r, qq, hh);
-            ok[k] = r < rows;
-            t[k] = (size_t)(c0 + qq);
-            query[k] = qq;
-            head[k] = kvh * p.G + hh;
-        }
-        // every pass's gates, requested before the first pass
-        uint4 gr[D / 64][RK];
-        if (p.gate) {
+            const float* src = out_stage + (8 * RK * kg + er + 8 * k) * S::RR + 8 * ec;
+            float y[8];
 #pragma unroll
-            for (int ps = 0; ps < D / 64; ps++)
+            for (int g = 0; g < KS; g++) {
+                const float4 a = *reinterpret_cast<const float4*>(src + g * (RG * 32 * S::RR)),
+                             b = *reinterpret_cast<const float4*>(src + g * (RG * 32 * S::RR) + 4);
+                const float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-                for (int k = 0; k < RK; k++)
-                    gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head +
-                                                                64 * ps + 8 * ec);
-        }
-        float inv;
-        if constexpr (SPLIT) {
-            float top = join[0][0][lq], sum = 0.f;
-#pragma unroll
-            for (int w = 1; w < NW; w++) top = fmaxf(top, join[w][0][lq]);
-            const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int w = 0; w < NW; w++) sum += join[w][1][lq] * __builtin_amdgcn_exp2f(join[w][0][lq] - base);
-            inv = __builtin_amdgcn_exp2f(m[0] - base) / sum;
-        } else {
-            inv = 1.f / add_xor32(l[qb]);
-        }
-#pragma unroll
-        for (int ps = 0; ps < D / 64; ps++) {
-#pragma unroll
-            for (int db = 2 * ps; db < 2 * ps + 2; db++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const f32x16& y = o[qb][db];
-                    *reinterpret_cast<float4*>(ew + lq * S::RR + 32 * (db - 2 * ps) + 8 * g + 4 * lh) =
-                        make_float4(y[4 * g] * inv, y[4 * g + 1] * inv, y[4 * g + 2] * inv, y[4 * g + 3] * inv);
-                }
-            if (SPLIT) __syncthreads();
-            else wave_sync();
-#pragma unroll
-            for (int k = 0; k < RK; k++) {
-                const float* src = (SPLIT ? reinterpret_cast<float*>(smem) : ew) + (r0 + er + 8 * k) * S::RR + 8 * ec;
-                float y[8];
-#pragma unroll
-                for (int w = 0; w < (SPLIT ? NW : 1); w++) {
-                    const float4 a = *reinterpret_cast<const float4*>(src + w * 32 * S::RR),
-                                 b = *reinterpret_cast<const float4*>(src + w * 32 * S::RR + 4);
-                    const float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = w == 0 ? z[i] : y[i] + z[i];
-                }
-                if (any_odd) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        if (query[k] >= odd[64 * ps + 8 * ec + i]) y[i] += INFINITY;
-                        if (query[k] >= odd[D + 64 * ps + 8 * ec + i]) y[i] -= INFINITY;
-                    }
-                }
-                if (p.gate) {
-                    const uint4 g = gr[ps][k];
-                    const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        y[2 * i] *= sigmoid(E::lo(gw[i]));
-                        y[2 * i + 1] *= sigmoid(E::hi(gw[i]));
-                    }
-                }
-                if (ok[k])
-                    *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + 64 * ps + 8 * ec) =
-                        make_uint4(E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7]));
+                for (int i = 0; i < 8; i++) y[i] = g == 0 ? z[i] : y[i] + z[i];
             }
-            // the region is rewritten by the next pass
-            if (SPLIT) __syncthreads();
-            else wave_sync();
+            if (any_odd) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (query[k] >= odd[64 * ps + 8 * ec + i]) y[i] += INFINITY;
+                    if (query[k] >= odd[D + 64 * ps + 8 * ec + i]) y[i] -= INFINITY;
+                }
+            }
+            if (p.gate) {
+                const uint4 g = gr[ps][k];
+                const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    y[2 * i] *= sigmoid(E::lo(gw[i]));
+                    y[2 * i + 1] *= sigmoid(E::hi(gw[i]));
+                }
+            }
+            if (ok[k])
+                *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + 64 * ps + 8 * ec) =
+                    make_uint4(E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7]));
         }
+        // the region is rewritten by the next pass
+        if (KS > 1) __syncthreads();
+        else wave_sync();
     }
 }
 
 // 1-D grid of at least (tiles of the batch) x Hkv workgroups, kv heads first:
 // workgroup ids go to the 8 XCDs in turn, so with 1, 2, 4 or a multiple of 8
 // kv heads an XCD reads the K and V of few heads through its L2.
-template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT, int OCC>
-__global__ void __launch_bounds__(64 * NW, OCC) packed_kernel(PackedParams p) {
-    using S = PackedTile<D, NQB, KB, NW, NST, SPLIT>;
+template <class E, int D, int RG, int KS, int NST, int OCC>
+__global__ void __launch_bounds__(64 * RG * KS, OCC) packed_kernel(PackedParams p) {
+    using S = PackedTile<D, RG, KS, NST>;
     __shared__ __align__(16) char smem[S::LDS];
     __shared__ int odd[2 * D + 1];
     const int kvh = blockIdx.x % p.Hkv;
     int c0, n, x;
-    if (!find_packed_tile<S::RW, NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
+    if (!find_packed_tile<S::RW, S::NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
     c0 = __builtin_amdgcn_readfirstlane(c0);  // scalars, for the requests' bases
     n = __builtin_amdgcn_readfirstlane(n);
     x = __builtin_amdgcn_readfirstlane(x);
-    packed_tile<E, D, NQB, KB, NW, NST, SPLIT>(p, smem, odd, c0, n, x, kvh);
+    packed_tile<E, D, RG, KS, NST>(p, smem, odd, c0, n, x, kvh);
 }
 
 }  // namespace pkv

@@ -12,26 +12,66 @@ int64_t tile_bound(const pkv::PackedParams& p, int rw) {
     return ((int64_t)p.T * p.G + rw - 1) / rw + std::min(p.seqs, p.T);
 }
 
-template <class E, int D, int NQB, int KB, int NW, int NST, bool SPLIT, int OCC>
+template <class E, int D, int RG, int KS, int NST, int OCC>
 int launch(const pkv::PackedParams& p, hipStream_t stream) {
-    using S = pkv::PackedTile<D, NQB, KB, NW, NST, SPLIT>;
+    using S = pkv::PackedTile<D, RG, KS, NST>;
     const int64_t grid = tile_bound(p, S::RW) * p.Hkv;
     if (grid * S::THREADS >= (int64_t)1 << 32) return PKV_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((pkv::packed_kernel<E, D, NQB, KB, NW, NST, SPLIT, OCC>), dim3((unsigned)grid), dim3(S::THREADS), 0,
-                       stream, p);
+    hipLaunchKernelGGL((pkv::packed_kernel<E, D, RG, KS, NST, OCC>), dim3((unsigned)grid), dim3(S::THREADS), 0, stream, p);
     return launch_status();
+}
+
+// How the rows and keys are shared out, by an estimate of the time in key tiles
+// of 32. RG waves with 32 rows each, KS times over for the keys: a workgroup's
+// time is its share of the tiles plus A tiles' worth of start and end, at the
+// mean length n = T / seqs, and the grid takes the longest workgroup or, where
+// it holds more than the card's places, the places' turns at the mean (half the
+// keys, causal). Measured, us, for 1 x 4, 2 x 2 and 4 x 1 (RG x KS): 256 dims at
+// 16 / 4 heads, one prompt of 600 tokens 22 / 25 / 31, 1,200 47 / 39 / 52, 2,400
+// 118 / 104 / 96, 20 of 60 31 / 23 / 14; 128 dims at 32 / 8, 500 11 / 13 / 17,
+// 1,200 33 / 25 / 33, 16 of 200 49 / 32 / 22; 64 dims at 12 / 2, 2,000 18 / 22 /
+// 38, 4,000 48 / 45 / 73. The estimate takes the fastest, or one within 16 %, in
+// all 29 batches that were timed.
+struct Shape {
+    int rows, ks, places;  // rows of a workgroup, key groups, workgroups a CU holds
+};
+int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[3], double start) {
+    const double tiles = (double)p.T / p.seqs / 32;
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 3; i++) {
+        const Shape& s = shapes[i];
+        const double turns = (double)tile_bound(p, s.rows) * p.Hkv / ((double)s.places * device_cus());
+        const double t = std::max(tiles / s.ks + start, turns * (tiles / (2 * s.ks) + start));
+        if (i == 0 || t < least) best = i, least = t;
+    }
+    return best;
 }
 
 template <class E>
 int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
-    if (tile_bound(p, 128) * p.Hkv < 128) {
-        if (D == 64) return launch<E, 64, 1, 1, 4, 2, true, 1>(p, stream);
-        if (D == 128) return launch<E, 128, 1, 1, 4, 1, true, 2>(p, stream);
-        return launch<E, 256, 1, 1, 4, 1, true, 1>(p, stream);
+    if (D == 64) {
+        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 4}, {128, 1, 4}};
+        switch (best_shape(p, shapes, 10)) {
+            case 0: return launch<E, 64, 1, 4, 2, 1>(p, stream);
+            case 1: return launch<E, 64, 2, 2, 2, 4>(p, stream);
+            default: return launch<E, 64, 4, 1, 2, 4>(p, stream);
+        }
     }
-    if (D == 64) return launch<E, 64, 1, 1, 4, 2, false, 4>(p, stream);
-    if (D == 128) return launch<E, 128, 1, 1, 4, 2, false, 3>(p, stream);
-    return launch<E, 256, 1, 1, 4, 2, false, 2>(p, stream);
+    if (D == 128) {
+        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 2}, {128, 1, 3}};
+        switch (best_shape(p, shapes, 20)) {
+            case 0: return launch<E, 128, 1, 4, 1, 2>(p, stream);
+            case 1: return launch<E, 128, 2, 2, 2, 2>(p, stream);
+            default: return launch<E, 128, 4, 1, 2, 3>(p, stream);
+        }
+    }
+    static constexpr Shape shapes[3] = {{32, 4, 1}, {64, 2, 1}, {128, 1, 2}};
+    switch (best_shape(p, shapes, 25)) {
+        case 0: return launch<E, 256, 1, 4, 1, 1>(p, stream);
+        case 1: return launch<E, 256, 2, 2, 2, 1>(p, stream);
+        default: return launch<E, 256, 4, 1, 2, 2>(p, stream);
+    }
 }
 
 }  // namespace
