@@ -35,8 +35,17 @@ struct PackedParams {
     long q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, o_row, o_head;
     const int* cu;
     int seqs, T, Hkv, G;
+    uint32_t g_mul;  // query of a row: its number divided by G (div_group)
+    int g_shift;
     float scale2;  // scale * log2(e)
 };
+
+// r / G for 0 <= r < 2^31 by one product (Granlund and Montgomery): with l =
+// ceil(log2 G) and g_mul = floor(2^(31 + l) / G) + 1, the error of r g_mul /
+// 2^(31 + l) stays below 1 / G. g_shift = 31 + l.
+__device__ __forceinline__ int div_group(const PackedParams& p, int r) {
+    return (int)(((uint64_t)(uint32_t)r * p.g_mul) >> p.g_shift);
+}
 
 // Shapes of a workgroup for heads of D dims: RG x KS waves, RG of them with 32
 // rows each, KS times over: key group g of KS takes the 32-key tiles g, g + KS,
@@ -55,11 +64,14 @@ struct PackedTile {
     static constexpr int KG = D == 256 ? 1040 : 1056, VG = 1088;
     static constexpr int STAGE = NG * (KG + VG);
     static constexpr int PER = NG / RG;  // groups of K (and of V) that a wave requests per tile
-    static constexpr int RR = 68;        // staged output row, floats of 64 dims
+    // Output passes of PW dims, rows staged in f32 (RR floats apart). 32 dims at
+    // 64, where the stages are small and more workgroups fit a CU with less.
+    static constexpr int PW = D == 64 && KS < 4 ? 32 : 64, RR = PW + 4;
     static constexpr int EPI = NW * 32 * RR * 4;
+    static constexpr int LPR = PW / 8, RPI = 64 / LPR;  // lanes per row, rows a wave writes at once
     static constexpr int STAGES = NST * KS * STAGE;
     static constexpr int LDS = STAGES > EPI ? STAGES : EPI;
-    static_assert(NG % RG == 0 && 4 % KS == 0, "whole groups a wave, whole 8-row pieces a key group");
+    static_assert(NG % RG == 0 && 32 % (RPI * KS) == 0, "whole groups a wave, whole pieces of rows a key group");
     static_assert(NST == 2 || (RG == 1 && NST == 1), "two stages, or one where a wave has it for itself");
     static __device__ __forceinline__ constexpr int swap(int r) { return D == 256 ? 0 : (r >> 3) & 1; }
 };
@@ -227,14 +239,14 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     // its last one and are not written.
     auto split = [&](int r, int& qi, int& hh) {
         r = min(r, rows - 1);
-        qi = r / p.G;
+        qi = div_group(p, r);
         hh = r - qi * p.G;
     };
-    const int L = (min(row0 + S::RW, rows) - 1) / p.G + 1;  // keys of this tile
+    const int L = div_group(p, min(row0 + S::RW, rows) - 1) + 1;  // keys of this tile
     const int ntiles = (L + BK - 1) / BK;
-    const int first_q = row0 / p.G;                          // of the tile
-    const int wfirst = min(wrow, rows - 1) / p.G;            // of the wave
-    const int last = wrow < rows ? (min(wrow + 32, rows) - 1) / p.G : -1;  // the wave's last (no rows: none)
+    const int first_q = div_group(p, row0);                        // of the tile
+    const int wfirst = div_group(p, min(wrow, rows - 1));          // of the wave
+    const int last = wrow < rows ? div_group(p, min(wrow + 32, rows) - 1) : -1;  // the wave's last (no rows: none)
 
     // Requests of K and V rows, straight to LDS: the wave's PER groups of its
     // key group's tile, lane i bringing 16 bytes of row g + NG (i / (D / 8))
@@ -426,11 +438,11 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     }
 
     // Rows out: a lane holds 4-dim pieces of one row, so 32 columns are 32 rows
-    // and go through LDS (64 dims a pass, f32: the one rounding comes after the
-    // gate), and leave as 16-byte pieces, 8 lanes per row. With several key
+    // and go through LDS (PW dims a pass, f32: the one rounding comes after the
+    // gate), and leave as 16-byte pieces, LPR lanes per row. With several key
     // groups their sums, brought to the same maximum, are added there, each
     // group's wave finishing its part of the 32 rows.
-    constexpr int RK = 4 / KS;  // rows a lane writes
+    constexpr int PW = S::PW, RPI = S::RPI, RK = 32 / (RPI * KS);  // RK rows a lane
     __shared__ float join[KS > 1 ? NW : 1][2][32];
     if constexpr (KS > 1) {
         l = add_xor32(l);
@@ -441,14 +453,14 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     }
     __syncthreads();  // every wave is past the last tile's stage
     float* const out_stage = reinterpret_cast<float*>(smem) + rg * 32 * S::RR;  // key group g's: + g RG 32 RR
-    const int er = lane >> 3, ec = lane & 7;
+    const int er = lane / S::LPR, ec = lane % S::LPR;
     const bool any_odd = odd[2 * D] != 0;
     size_t t[RK];
     int head[RK], query[RK];
     bool ok[RK];
 #pragma unroll
     for (int k = 0; k < RK; k++) {
-        const int r = wrow + 8 * RK * kg + er + 8 * k;
+        const int r = wrow + RPI * RK * kg + er + RPI * k;
         int hh;
         split(r, query[k], hh);
         ok[k] = r < rows;
@@ -456,13 +468,13 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         head[k] = kvh * p.G + hh;
     }
     // every pass's gates, requested before the first pass
-    uint4 gr[D / 64][RK];
+    uint4 gr[D / PW][RK];
     if (p.gate) {
 #pragma unroll
-        for (int ps = 0; ps < D / 64; ps++)
+        for (int ps = 0; ps < D / PW; ps++)
 #pragma unroll
             for (int k = 0; k < RK; k++)
-                gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head + 64 * ps +
+                gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head + PW * ps +
                                                             8 * ec);
     }
     float inv;
@@ -478,13 +490,13 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         inv = 1.f / add_xor32(l);
     }
 #pragma unroll
-    for (int ps = 0; ps < D / 64; ps++) {
+    for (int ps = 0; ps < D / PW; ps++) {
 #pragma unroll
-        for (int db = 2 * ps; db < 2 * ps + 2; db++)
+        for (int db = PW / 32 * ps; db < PW / 32 * (ps + 1); db++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const f32x16& y = o[db];
-                *reinterpret_cast<float4*>(out_stage + kg * (RG * 32 * S::RR) + lq * S::RR + 32 * (db - 2 * ps) + 8 * g +
+                *reinterpret_cast<float4*>(out_stage + kg * (RG * 32 * S::RR) + lq * S::RR + 32 * (db - PW / 32 * ps) + 8 * g +
                                            4 * lh) =
                     make_float4(y[4 * g] * inv, y[4 * g + 1] * inv, y[4 * g + 2] * inv, y[4 * g + 3] * inv);
             }
@@ -492,7 +504,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         else wave_sync();
 #pragma unroll
         for (int k = 0; k < RK; k++) {
-            const float* src = out_stage + (8 * RK * kg + er + 8 * k) * S::RR + 8 * ec;
+            const float* src = out_stage + (RPI * (RK * kg + k) + er) * S::RR + 8 * ec;
             float y[8];
 #pragma unroll
             for (int g = 0; g < KS; g++) {
@@ -505,8 +517,8 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
             if (any_odd) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    if (query[k] >= odd[64 * ps + 8 * ec + i]) y[i] += INFINITY;
-                    if (query[k] >= odd[D + 64 * ps + 8 * ec + i]) y[i] -= INFINITY;
+                    if (query[k] >= odd[PW * ps + 8 * ec + i]) y[i] += INFINITY;
+                    if (query[k] >= odd[D + PW * ps + 8 * ec + i]) y[i] -= INFINITY;
                 }
             }
             if (p.gate) {
@@ -519,7 +531,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
                 }
             }
             if (ok[k])
-                *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + 64 * ps + 8 * ec) =
+                *reinterpret_cast<uint4*>(p.out + t[k] * p.o_row + (size_t)head[k] * p.o_head + PW * ps + 8 * ec) =
                     make_uint4(E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7]));
         }
         // the region is rewritten by the next pass

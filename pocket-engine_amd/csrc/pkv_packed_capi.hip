@@ -51,11 +51,11 @@ int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[3], double star
 template <class E>
 int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
     if (D == 64) {
-        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 4}, {128, 1, 4}};
+        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 4}, {128, 1, 5}};
         switch (best_shape(p, shapes, 10)) {
             case 0: return launch<E, 64, 1, 4, 2, 1>(p, stream);
             case 1: return launch<E, 64, 2, 2, 2, 4>(p, stream);
-            default: return launch<E, 64, 4, 1, 2, 4>(p, stream);
+            default: return launch<E, 64, 4, 1, 2, 5>(p, stream);
         }
     }
     if (D == 128) {
@@ -105,6 +105,10 @@ extern "C" int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, con
     p.g_row = gate_row, p.g_head = gate_head, p.o_row = out_row, p.o_head = out_head;
     p.cu = cu;
     p.seqs = seqs, p.T = T, p.Hkv = Hkv, p.G = Hq / Hkv;
+    int l = 0;
+    while (((int64_t)1 << l) < p.G) l++;
+    p.g_shift = 31 + l;
+    p.g_mul = (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)p.G + 1);
     p.scale2 = scale * pkv::LOG2E;
     return dtype == PKV_BF16 ? by_dims<pkv::Bf16>(p, D, (hipStream_t)stream)
                              : by_dims<pkv::Fp16>(p, D, (hipStream_t)stream);
