@@ -295,7 +295,10 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
         for (int kk = 0; kk < D / 16; kk++) qf[kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
     }
     f32x16 o[D / 32];
-    float m = -INFINITY, l = 0.f;  // running maximum (log2 units, may lag, below); the lane's own part of the sum
+    // running maximum (log2 units; 0 before the first key; may lag, below) and
+    // the lane's own part of the sum
+    float m = 0.f, l = 0.f, limit = -1.f;
+    bool fresh = true;  // uniform: some row of the wave has no key yet
 #pragma unroll
     for (int db = 0; db < D / 32; db++)
 #pragma unroll
@@ -322,40 +325,56 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
             for (int r = 0; r < 16; r++)
                 if (k0 + 8 * (r >> 2) + 4 * lh + (r & 3) > qi) st[r] = -INFINITY;
         }
-        float mx = st[0];
+        // Weights against the maximum as it stands. P is rounded to the type of
+        // the rows, as the matrix units take it; the sum is of the rounded
+        // weights, so they still add up to 1.
+        uint4 pb[2];
+        float sum;
+        auto weigh = [&](float base) __attribute__((always_inline)) {
+            sum = 0.f;
 #pragma unroll
-        for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[r]);
-        mx = max_xor32(mx) * p.scale2;
-        // The maximum may lag behind by up to 8: weights up to 2^8, all of a
-        // row relative to the same power, so no digit is lost, and the
-        // rescaling of O is skipped in almost every tile.
-        if (__any(mx > m + 8.f)) {
-            const float mn = fmaxf(m, mx);
-            const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-            m = mn;
+            for (int kk = 0; kk < 2; kk++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float s0 = st[8 * kk + 2 * i], s1 = st[8 * kk + 2 * i + 1];
+                    w[i] = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.scale2, -base)),
+                                   __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.scale2, -base)));
+                    sum = E::dot(w[i], E::ONE, sum);
+                }
+                pb[kk] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        };
+        // The maximum is looked for only before a row's first key (`limit` is
+        // -1) and where the tile's weights outgrow it (a lane's 16 add up to
+        // more than 2^10): weights up to 2^10, all of a row relative to the
+        // same power, lose no digit, and almost every tile is spared the
+        // search, the rescaling of O and the wait for both between the two
+        // products.
+        bool search = fresh;
+        if (!fresh) {
+            weigh(m);
+            search = __any(sum > limit);
+        }
+        if (search) {
+            float mx = st[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) mx = fmaxf(mx, st[r]);
+            mx = fmaxf(max_xor32(mx) * p.scale2, limit < 0.f ? -INFINITY : m);
+            // scores of -inf so far: their weight is 0, not NaN
+            const float base = mx == -INFINITY ? 0.f : mx;
+            const float corr = limit < 0.f ? 0.f : __builtin_amdgcn_exp2f(m - base);
+            m = base;
+            limit = mx == -INFINITY ? -1.f : 1024.f;
+            fresh = __any(limit < 0.f);
             l *= corr;
 #pragma unroll
             for (int db = 0; db < D / 32; db++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[db][r] *= corr;
+            weigh(m);
         }
-        // scores of -inf so far: their weight is 0, not NaN
-        const float base = m == -INFINITY ? 0.f : m;
-        // P is rounded to the type of the rows, as the matrix units take it;
-        // the sum is of the rounded weights, so they still add up to 1.
-        uint4 pb[2];
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float s0 = st[8 * kk + 2 * i], s1 = st[8 * kk + 2 * i + 1];
-                w[i] = E::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.scale2, -base)),
-                               __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.scale2, -base)));
-                l = E::dot(w[i], E::ONE, l);
-            }
-            pb[kk] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        l += sum;
 #pragma unroll
         for (int kk = 0; kk < 2; kk++)
 #pragma unroll
@@ -447,7 +466,7 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     if constexpr (KS > 1) {
         l = add_xor32(l);
         if (lh == 0) {
-            join[wave][0][lq] = m;
+            join[wave][0][lq] = limit < 0.f ? -INFINITY : m;  // no key yet
             join[wave][1][lq] = l;
         }
     }
@@ -479,13 +498,13 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     }
     float inv;
     if constexpr (KS > 1) {
-        float top = m, sum = 0.f;
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int g = 0; g < KS; g++) top = fmaxf(top, join[g * RG + rg][0][lq]);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int g = 0; g < KS; g++) sum += join[g * RG + rg][1][lq] * __builtin_amdgcn_exp2f(join[g * RG + rg][0][lq] - base);
-        inv = __builtin_amdgcn_exp2f(m - base) / sum;
+        inv = __builtin_amdgcn_exp2f(join[wave][0][lq] - base) / sum;
     } else {
         inv = 1.f / add_xor32(l);
     }
