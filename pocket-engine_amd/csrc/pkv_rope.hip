@@ -149,70 +149,104 @@ __device__ __forceinline__ float2 turn_of(int pos, float inv) {
 // A lane takes 16 dims of a head as two 16-byte pieces: where they are
 // rotated, the pieces whose dims pair up (half-split pairs (i, i + half)) or
 // any two (adjacent pairs (2 i, 2 i + 1)), so no value crosses lanes; D / 16
-// lanes share a head and its norm's sum. The cos / sin of TB tokens are made
-// once per workgroup, in LDS, and stay in registers over a token's heads.
-template <class E, int D, bool ADJ, int TB>
-__global__ void __launch_bounds__(256) rope_rows_kernel(RopeParams p) {
-    __shared__ __align__(16) float cs[TB][2][D / 2];  // cos, sin
-    constexpr int LPH = D / 16, HPB = 256 / LPH;      // lanes per head, heads at a time
-    const int tid = threadIdx.x, t0 = blockIdx.x * TB, u = tid % LPH, slot = tid / LPH;
-    const int H = p.Hq + p.Hkv;
-    for (int i = tid; i < TB * p.half; i += 256) {
-        const int tt = i / p.half, f = i - tt * p.half, t = t0 + tt;
-        if (t < p.T) {
-            int axis = p.axes[f];
-            axis = axis == 1 || axis == 2 ? axis : 0;
-            const float2 y = turn_of(p.rope[(size_t)axis * p.rope_stride + t], p.inv_freq[f]);
-            cs[tt][0][f] = y.x;
-            cs[tt][1][f] = y.y;
-        }
-    }
-    __syncthreads();
-    const int pieces = p.half / 8;       // pairs of pieces that are rotated
+// lanes share a head and its norm's sum. A workgroup takes the heads of `tb`
+// tokens, its threads going through the (token, head) pairs HPB at a time; the
+// tokens' cos / sin are made once, in LDS, while the first pair's rows are on
+// their way.
+constexpr int ROPE_TOKENS = 8;  // tb at most
+template <class E, int D, bool ADJ, bool STREAM>
+__global__ void __launch_bounds__(256) rope_rows_kernel(RopeParams p, int tb) {
+    __shared__ __align__(16) float cs[ROPE_TOKENS][2][D / 2];  // cos, sin
+    constexpr int LPH = D / 16, HPB = 256 / LPH;               // lanes per head, heads at a time
+    const int tid = threadIdx.x, t0 = blockIdx.x * tb, u = tid % LPH;
+    const int H = p.Hq + p.Hkv, tokens = min(tb, p.T - t0);
+    const int pieces = p.half / 8;  // pairs of pieces that are rotated
     const bool turned = u < pieces;
     const int d0 = 8 * (turned ? u : 2 * u), d1 = 8 * (turned ? u + pieces : 2 * u + 1);
-    for (int tt = 0; tt < TB; tt++) {
-        const int t = t0 + tt;
-        if (t >= p.T) break;
-        float c[8], s[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // adjacent: frequencies of the first piece's 4 pairs, then of the second's
-            const int f = ADJ ? (i < 4 ? d0 / 2 + i : d1 / 2 + i - 4) : d0 + i;
-            c[i] = turned ? cs[tt][0][f] : 1.f;
-            s[i] = turned ? cs[tt][1][f] : 0.f;
+    // the (token, head) pair of this thread, and its rows
+    int tt = 0, hh = tid / LPH;
+    while (hh >= H && tt < tokens) hh -= H, tt++;
+    uint4 ra, rb;
+    auto load = [&]() {
+        const size_t t = t0 + tt;
+        const uint16_t* src = hh < p.Hq ? p.q + t * p.q_row + (size_t)hh * p.q_head
+                                        : p.k + t * p.k_row + (size_t)(hh - p.Hq) * p.k_head;
+        ra = *reinterpret_cast<const uint4*>(src + d0);
+        rb = *reinterpret_cast<const uint4*>(src + d1);
+    };
+    // Angles of (token j, pair f), D / 2 threads a token, of which `half` have
+    // a pair; all three axes at once, so that no load waits for the axis.
+    struct Angle {
+        int time, height, width, axis;
+        float inv;
+    };
+    auto angle = [&](int j, int f) {
+        const int* at = p.rope + t0 + j;
+        return Angle{at[0], at[p.rope_stride], at[2 * (size_t)p.rope_stride], p.axes[f], p.inv_freq[f]};
+    };
+    auto keep = [&](const Angle& y, int j, int f) {
+        const float2 r = turn_of(y.axis == 1 ? y.height : y.axis == 2 ? y.width : y.time, y.inv);
+        cs[j][0][f] = r.x;
+        cs[j][1][f] = r.y;
+    };
+    if (p.half > 0) {
+        // the first round's loads stand before those of the rows: loads return
+        // in order, and the angles are worked out while the rows come
+        constexpr int STEP = 256 / (D / 2);  // tokens a round
+        const int f = tid % (D / 2), j = tid / (D / 2);
+        const Angle y = angle(min(j, tokens - 1), min(f, p.half - 1));
+        if (tt < tokens) load();
+        if (f < p.half) {
+            if (j < tokens) keep(y, j, f);
+            for (int i = j + STEP; i < tokens; i += STEP) keep(angle(i, f), i, f);
         }
-        for (int hh = slot; hh < H; hh += HPB) {
-            const bool is_q = hh < p.Hq;
-            const uint16_t* src = is_q ? p.q + (size_t)t * p.q_row + (size_t)hh * p.q_head
-                                       : p.k + (size_t)t * p.k_row + (size_t)(hh - p.Hq) * p.k_head;
-            uint16_t* dst = is_q ? p.q_out + (size_t)t * p.qo_row + (size_t)hh * p.qo_head
-                                 : p.k_out + (size_t)t * p.ko_row + (size_t)(hh - p.Hq) * p.ko_head;
-            const uint4 ra = *reinterpret_cast<const uint4*>(src + d0), rb = *reinterpret_cast<const uint4*>(src + d1);
-            const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
-            float a[8], b[8];
+    } else if (tt < tokens) {
+        load();
+    }
+    __syncthreads();
+    while (tt < tokens) {
+        const int t = t0 + tt;
+        const bool is_q = hh < p.Hq;
+        uint16_t* dst = is_q ? p.q_out + (size_t)t * p.qo_row + (size_t)hh * p.qo_head
+                             : p.k_out + (size_t)t * p.ko_row + (size_t)(hh - p.Hq) * p.ko_head;
+        const uint32_t wa[4] = {ra.x, ra.y, ra.z, ra.w}, wb[4] = {rb.x, rb.y, rb.z, rb.w};
+        float a[8], b[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                a[2 * i] = E::lo(wa[i]);
-                a[2 * i + 1] = E::hi(wa[i]);
-                b[2 * i] = E::lo(wb[i]);
-                b[2 * i + 1] = E::hi(wb[i]);
+        for (int i = 0; i < 4; i++) {
+            a[2 * i] = E::lo(wa[i]);
+            a[2 * i + 1] = E::hi(wa[i]);
+            b[2 * i] = E::lo(wb[i]);
+            b[2 * i + 1] = E::hi(wb[i]);
+        }
+        const int row = tt;
+        // the next pair's rows are requested before this one is worked on
+        hh += HPB;
+        while (hh >= H && tt < tokens) hh -= H, tt++;
+        if (tt < tokens) load();
+        const float* w = is_q ? p.q_norm : p.k_norm;
+        if (w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+            for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o);
+            const float sc = 1.f / sqrtf(ss / D + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                a[i] *= sc * w[d0 + i];
+                b[i] *= sc * w[d1 + i];
             }
-            const float* w = is_q ? p.q_norm : p.k_norm;
-            if (w) {
-                float ss = 0.f;
+        }
+        uint32_t oa[4], ob[4];
+        if (turned) {
+            float c[8], s[8];
+            // adjacent: frequencies of the first piece's 4 pairs, then of the second's
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-                for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o);
-                const float sc = 1.f / sqrtf(ss / D + p.eps);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    a[i] *= sc * w[d0 + i];
-                    b[i] *= sc * w[d1 + i];
-                }
+            for (int i = 0; i < 8; i += 4) {
+                const int f = ADJ ? (i ? d1 : d0) / 2 : d0 + i;
+                *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(&cs[row][0][f]);
+                *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(&cs[row][1][f]);
             }
-            uint32_t oa[4], ob[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if constexpr (ADJ) {
@@ -225,15 +259,21 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RopeParams p) {
                     ob[i] = E::pack(b[j] * c[j] + a[j] * s[j], b[j + 1] * c[j + 1] + a[j + 1] * s[j + 1]);
                 }
             }
-            if (!turned) {  // as they are (normed): 0 x infinity must not enter
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    oa[i] = E::pack(a[2 * i], a[2 * i + 1]);
-                    ob[i] = E::pack(b[2 * i], b[2 * i + 1]);
-                }
+            for (int i = 0; i < 4; i++) {
+                oa[i] = E::pack(a[2 * i], a[2 * i + 1]);
+                ob[i] = E::pack(b[2 * i], b[2 * i + 1]);
             }
-            *reinterpret_cast<uint4*>(dst + d0) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-            *reinterpret_cast<uint4*>(dst + d1) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+        }
+        const u32x4 ya = {oa[0], oa[1], oa[2], oa[3]}, yb = {ob[0], ob[1], ob[2], ob[3]};
+        u32x4 *pa = reinterpret_cast<u32x4*>(dst + d0), *pb = reinterpret_cast<u32x4*>(dst + d1);
+        if constexpr (STREAM) {
+            __builtin_nontemporal_store(ya, pa);
+            __builtin_nontemporal_store(yb, pb);
+        } else {
+            *pa = ya;
+            *pb = yb;
         }
     }
 }
