@@ -11,6 +11,7 @@
 // row then needs the last span at or before it (rope_positions).
 #pragma once
 #include "pkv_rows.h"
+#include "pkv_wave.h"
 
 namespace pkv {
 
@@ -24,17 +25,6 @@ __device__ __forceinline__ SpanSize span_size(int t, int h, int w, int step) {
     const long hw = (long)h * w, time = (long)(t - 1) * step + 1;
     if (hw > 0x7fffffff || hw * t > 0x7fffffff || time > 0x7fffffff) return {0, 0};
     return {(int)(hw * t), max((int)time, max(h, w))};
-}
-
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
 }
 
 // A workgroup of NW waves per request: the prefix sum in rounds of 64 NW
@@ -57,7 +47,7 @@ __global__ void __launch_bounds__(64 * NW) rope_spans_kernel(const int* __restri
             const SpanSize z = span_size(sp[1], sp[2], sp[3], sp[4]);
             gain = (unsigned)z.extent - (unsigned)z.count;
         }
-        const unsigned incl = (unsigned)wave_scan((int)gain);
+        const unsigned incl = (unsigned)wave_prefix((int)gain);
         unsigned before = carry;
         if constexpr (NW > 1) {
             // (two turns of `part`: a wave a round ahead writes the other one)
@@ -69,7 +59,7 @@ __global__ void __launch_bounds__(64 * NW) rope_spans_kernel(const int* __restri
                 carry += (unsigned)part[turn][w];
             }
         } else {
-            carry += (unsigned)__shfl((int)incl, 63);
+            carry += (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
         }
         if (i < b) base[i] = (int)((unsigned)start + before + incl - gain);
     }

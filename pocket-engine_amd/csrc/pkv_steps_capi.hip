@@ -5,6 +5,8 @@
 #include "pkv_rope.hip"
 #include "pkv_entry.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int64_t INT_LIMIT = 0x7fffffff;
@@ -76,11 +78,20 @@ int pkv_plan_step(const int32_t* len, const int32_t* held, const int32_t* ntok, 
     p.free_list = free_list, p.free_count = free_count, p.T = T;
     p.pos = pos, p.slot_map = slot_map, p.tok_seq = tok_seq, p.cu = cu, p.limits = limits;
     p.len_out = len_out, p.held_out = held_out, p.free_out = free_count_out, p.status = status;
-    if (T <= 2048 || nrows == 0) {
-        hipLaunchKernelGGL(pkv::plan_rows_kernel<true>, dim3(1), dim3(pkv::PLAN_THREADS), 0, (hipStream_t)stream, p);
+    // 256 threads where they hold the rows and, one workgroup, the tokens in two
+    // turns (64 rows 6.9 -> 4.2 us).
+    const bool in_place = len_out == len || held_out == held || (free_count_out && free_count_out == free_count);
+    const bool one = in_place && (T <= 2048 || nrows == 0), small = nrows <= 256 && (!one || T <= 512);
+    const int threads = small ? 256 : 1024;
+    const dim3 grid(in_place ? 1 : std::max(1, std::min(256, (T + threads - 1) / threads)));
+    const hipStream_t hs = (hipStream_t)stream;
+    if (one || !in_place) {
+        hipLaunchKernelGGL((small ? pkv::plan_rows_kernel<true, 4> : pkv::plan_rows_kernel<true, 16>), grid, dim3(threads), 0,
+                           hs, p);
         return launch_status();
     }
-    hipLaunchKernelGGL(pkv::plan_rows_kernel<false>, dim3(1), dim3(pkv::PLAN_THREADS), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((small ? pkv::plan_rows_kernel<false, 4> : pkv::plan_rows_kernel<false, 16>), grid, dim3(threads), 0,
+                       hs, p);
     const int s = launch_status();
     if (s != PKV_OK) return s;
     hipLaunchKernelGGL(pkv::plan_tokens_kernel, dim3((T + 255) / 256), dim3(256), 0, (hipStream_t)stream, p);
@@ -97,7 +108,7 @@ int pkv_plan_truncate(const int32_t* new_len, int32_t* len, int32_t* held, int n
     p.new_len = new_len, p.len = len, p.held = held, p.nrows = nrows;
     p.table = block_table, p.max_blocks = max_blocks, p.block_size = block_size, p.num_blocks = (int)num_blocks;
     p.free_list = free_list, p.free_count = free_count;
-    hipLaunchKernelGGL(pkv::plan_truncate_kernel, dim3(1), dim3(pkv::PLAN_THREADS), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(pkv::plan_truncate_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p);
     return launch_status();
 }
 

@@ -368,7 +368,7 @@ def _launch(what, fn, dev, stream, *args):
         stream = torch._C._cuda_getCurrentRawStream(dev)
     elif not isinstance(stream, int):
         stream = stream.cuda_stream
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         status = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
