@@ -297,3 +297,24 @@ def test_two_streams_and_repeats(dev):
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([900], 4, 1), ([1500], 16, 4), ([250] * 8, 16, 4), ([2600], 8, 1),
+                                         ([3, 1, 2] * 40, 3, 3)])
+def test_every_shape_of_workgroup(dev, D, lens, Hq, Hkv):
+    """Batches that are shared out among a workgroup's waves by keys, by both and by rows."""
+    c = inputs(lens, Hq, Hkv, D, "bf16", D + len(lens), dev, gate=D == 256)
+    check(c, run(c), f"D {D} {len(lens)} x {lens[0]} heads {Hq}/{Hkv}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scores_that_jump(dev, dtype):
+    """A key now and then scores far above all before it, in tiles of any key group, for some rows only."""
+    for D, n in ((64, 700), (128, 333), (256, 130)):
+        c = inputs([n], 4, 1, D, dtype, n, dev, amp=0.3)
+        c["q"][::3, :, 0] = 4.0
+        c["k"][:, :, 0] = 0.0
+        for i, at in enumerate(range(5, n, 41)):
+            c["k"][at, :, 0] = 3.0 * D ** 0.5 * (i + 1) / 4  # 3 (i + 1) above the others in score
+        check(c, run(c), f"{dtype} D {D}")

@@ -219,3 +219,21 @@ def test_no_heads_and_replay(dev):
         w = rows_check(c)
         torch.cuda.synchronize()
         assert torch.equal(qo, w[0]) and torch.equal(ko, w[1])
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(17000, 32, 8, 128), (9000, 2, 1, 64), (5000, 16, 4, 256)])
+def test_many_rows_are_the_same_rows(dev, T, Hq, Hkv, D):
+    """Several tokens to a workgroup and outputs past the caches: bit for bit what short calls give, also at an odd end."""
+    g = torch.Generator(device=dev).manual_seed(T)
+    q, k = (torch.randn(T, h, D, device=dev, generator=g).bfloat16() for h in (Hq, Hkv))
+    rope = torch.randint(0, 100000, (3, T), device=dev, generator=g, dtype=torch.int32)
+    axes = torch.arange(D // 2, device=dev, dtype=torch.int32) % 3
+    inv = (1e6 ** (-torch.arange(D // 2, device=dev) / (D // 2))).float()
+    w = 1 + 0.1 * torch.randn(D, device=dev, generator=g)
+    qo, ko = torch.full_like(q, 9), torch.full_like(k, 9)
+    pkv.rope_rows(q, k, rope, axes, inv, qo, ko, q_norm=w)
+    for a, b in ((0, 700), (T // 2, T // 2 + 333), (T - 411, T)):
+        sq, sk = torch.zeros_like(q[a:b]), torch.zeros_like(k[a:b])
+        pkv.rope_rows(q[a:b], k[a:b], rope[:, a:b].contiguous(), axes, inv, sq, sk, q_norm=w)
+        assert torch.equal(qo[a:b], sq) and torch.equal(ko[a:b], sk)
+    assert not (qo == 9).all(-1).any() and not (ko == 9).all(-1).any()
