@@ -423,8 +423,8 @@ int pkv_rope_positions(const int32_t* pos, const int32_t* tok_seq, int T, const 
  * axis of pair i (values other than 1 and 2: time), so any sections of axes,
  * one after the other or interleaved. Angles are exact to 2^-40 of a turn at
  * any position, the arithmetic is f32, rounded once at the end (pkv_attn_prep
- * rounds where the reference does). Rows and strides as pkv_attn_packed; out
- * may be in (same strides), else they may not overlap. rot is a multiple of 16
+ * rounds where the reference does). Rows and strides as pkv_attn_packed; each
+ * out may be its input (same strides), else they may not overlap. rot is a multiple of 16
  * (0: norm alone). Hq or Hkv may be 0. */
 int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                   void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row,
@@ -446,15 +446,19 @@ int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, i
  * Rows of D = 64, 128 or 256 contiguous elements of dtype (PKV_BF16,
  * PKV_FP16); *_row and *_head are the strides in elements between rows
  * (tokens) and between heads, multiples of 8, 0 .. 2^24 (the views of a
- * projection row [Hq x (q | gate) | k | v] as they are; out rows may not
- * overlap, nor overlap inputs). Pointers 16-byte aligned. Scores, sums and
- * values in f32; weights are rounded to dtype for the second product and the
- * output once, after the gate. Rows outside every sequence are left as they
- * are; an empty sequence is skipped; offsets outside [0, T] are clamped. An
- * infinite or NaN value, key or query reaches exactly the rows that attend
- * it. scale is finite and above 0. PKV_ERR_UNSUPPORTED for other types, dims
- * or groups, or T G above 2^30. No workspace. No reference counterpart (the
- * reference attends through its pages only, src/model.rs:2438-2493). */
+ * projection row [Hq x (q | gate) | k | v] as they are); out's rows lie inside
+ * its heads or its heads inside its rows. out may be q or gate, with their
+ * strides, and may not overlap the inputs otherwise. Pointers 16-byte aligned.
+ * Scores, sums and values in f32; weights are rounded to dtype for the second
+ * product and the output once, after the gate (0 for gates below -87.3). Rows
+ * outside every sequence are left as they are; an empty sequence is skipped;
+ * offsets outside [0, T] are clamped. An infinite or NaN value, key or query
+ * reaches exactly the rows that attend it. The same call gives the same bits;
+ * how a batch's keys are shared out, and with it the last bits of a row, goes
+ * by T, seqs and the heads. scale is finite and above 0. PKV_ERR_UNSUPPORTED
+ * for other types, dims or groups, or T G above 2^30. No workspace. No
+ * reference counterpart (the reference attends through its pages only,
+ * src/model.rs:2438-2493). */
 int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                     const void* v, int64_t v_row, int64_t v_head, const void* gate, int64_t gate_row,
                     int64_t gate_head, void* out, int64_t out_row, int64_t out_head, const int32_t* cu, int seqs, int T,

@@ -15,6 +15,16 @@ inline int launch_status() { return status_of(hipGetLastError()); }
 
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
+// Strides of rows of 16-byte pieces: multiples of 8 elements, 0 .. 2^24.
+inline bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s <= ((int64_t)1 << 24); }
+
+// T rows of H heads of D elements that are written lie apart: the heads inside
+// a row's stride or the rows inside a head's.
+inline bool apart(int64_t row, int64_t head, int T, int H, int D) {
+    const bool rows = T <= 1 || row >= D, heads = H <= 1 || head >= D;
+    return rows && heads && (T <= 1 || H <= 1 || row >= (H - 1) * head + D || head >= (T - 1) * row + D);
+}
+
 // Compute units of the current device, cached per device.
 inline int device_cus() {
     static std::atomic<int> cus[64];

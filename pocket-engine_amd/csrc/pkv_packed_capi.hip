@@ -89,11 +89,10 @@ extern "C" int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, con
     const int64_t strides[] = {q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, gate ? gate_row : 0,
                                gate ? gate_head : 0};
     for (int64_t s : strides)
-        if (s < 0 || s % 8 != 0 || s > ((int64_t)1 << 24)) return PKV_ERR_INVALID;
+        if (!stride_ok(s)) return PKV_ERR_INVALID;
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(gate, 16))
         return PKV_ERR_INVALID;
-    // rows of their own for every token and head
-    if ((T > 1 && out_row < D) || (Hq > 1 && out_head < D)) return PKV_ERR_INVALID;
+    if (!apart(out_row, out_head, T, Hq, D)) return PKV_ERR_INVALID;
     if ((int64_t)T * (Hq / Hkv) > (int64_t)1 << 30) return PKV_ERR_UNSUPPORTED;
     pkv::PackedParams p;
     p.q = (const uint16_t*)q;

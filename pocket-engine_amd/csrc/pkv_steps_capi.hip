@@ -27,7 +27,7 @@ bool words(std::initializer_list<const void*> ps) {
 
 bool strides_ok(std::initializer_list<int64_t> ss) {
     for (int64_t s : ss)
-        if (s < 0 || s % 8 != 0 || s > ((int64_t)1 << 24)) return false;
+        if (!stride_ok(s)) return false;
     return true;
 }
 
@@ -143,12 +143,11 @@ int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, i
         return PKV_ERR_UNSUPPORTED;
     if (T == 0 || Hq + Hkv == 0) return PKV_OK;
     if (Hq > 0 && (!q || !q_out || !aligned(q, 16) || !aligned(q_out, 16) ||
-                   !strides_ok({q_row, q_head, q_out_row, q_out_head}) || (T > 1 && q_out_row < D) ||
-                   (Hq > 1 && q_out_head < D)))
+                   !strides_ok({q_row, q_head, q_out_row, q_out_head}) || !apart(q_out_row, q_out_head, T, Hq, D)))
         return PKV_ERR_INVALID;
     if (Hkv > 0 && (!k || !k_out || !aligned(k, 16) || !aligned(k_out, 16) ||
-                    !strides_ok({k_row, k_head, k_out_row, k_out_head}) || (T > 1 && k_out_row < D) ||
-                    (Hkv > 1 && k_out_head < D)))
+                    !strides_ok({k_row, k_head, k_out_row, k_out_head}) ||
+                    !apart(k_out_row, k_out_head, T, Hkv, D)))
         return PKV_ERR_INVALID;
     if (rot > 0 && (!words({rope, axes, inv_freq}) || rope_stride < T)) return PKV_ERR_INVALID;
     if (!aligned(q_norm, 4) || !aligned(k_norm, 4)) return PKV_ERR_INVALID;

@@ -318,3 +318,30 @@ def test_scores_that_jump(dev, dtype):
         for i, at in enumerate(range(5, n, 41)):
             c["k"][at, :, 0] = 3.0 * D ** 0.5 * (i + 1) / 4  # 3 (i + 1) above the others in score
         check(c, run(c), f"{dtype} D {D}")
+
+
+@pytest.mark.parametrize("which", ["q", "gate"])
+def test_out_may_be_the_queries_or_the_gates(dev, which):
+    for lens, D in (([100, 3], 64), ([300] * 9, 128), ([260], 256), ([200] * 30, 256)):
+        c = inputs(lens, 8, 2, D, "bf16", D, dev, gate=True)
+        want = run(c)
+        assert torch.equal(run(c, c[which]), want)
+
+
+def test_rows_past_2_gib(dev):
+    """Rows 32 KiB apart: the last ones start behind 2^31 bytes of every operand."""
+    T, H, D = 70000, 2, 64
+    x = torch.zeros(T, 16384, device=dev, dtype=torch.bfloat16)
+    part = lambda i: x[:, i * H * D:(i + 1) * H * D].view(T, H, D)
+    g = torch.Generator(device=dev).manual_seed(1)
+    for i in range(4):
+        part(i).copy_(torch.randn(T, H, D, device=dev, generator=g))
+    q, k, v, gate, out = (part(i) for i in range(5))
+    # the rows in between belong to no sequence
+    for cu in ([0, 1, 701], [69700, 70000]):
+        pkv.attn_packed(q, k, v, torch.tensor(cu, dtype=torch.int32, device=dev), out, 0.125, gate=gate)
+    for a, b in ((1, 701), (69700, 70000)):
+        c = dict(q=q[a:b].contiguous(), k=k[a:b].contiguous(), v=v[a:b].contiguous(), gate=gate[a:b].contiguous(),
+                 cu=torch.tensor([0, b - a], dtype=torch.int32, device=dev), lens=[b - a], lead=0, scale=0.125)
+        check(c, out[a:b], f"rows {a}..{b}")
+    assert (out[701:69700] == 0).all() and (x[:, 5 * H * D:] == 0).all()

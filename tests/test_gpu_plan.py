@@ -332,3 +332,54 @@ def test_the_operators_together(dev):
     last = fo[fcu[1:].long() - 1]
     assert ((o1.float() - last.float()).abs() <= near).all()
     assert (o1.float() - last.float()).norm() <= 0.02 * last.float().norm()
+
+
+def test_a_captured_prompt_step(dev):
+    """Plan, positions, rows and attention of a batch of prompts captured once, replayed for other lengths and values
+    with eager calls between: every replay equal to the eager run of the same step."""
+    n, T, Hq, Hkv, D, bs, pool, width = 5, 400, 8, 2, 128, 16, 80, 30
+    g = torch.Generator(device=dev).manual_seed(9)
+    new = lambda *k: torch.zeros(*k, dtype=torch.int32, device=dev)
+    rows = lambda h: torch.zeros(T, h, D, device=dev, dtype=torch.bfloat16)
+    scu, spans = i32([0, 1, 1, 3, 3, 3], dev), i32([[4, 1, 3, 5, 1], [0, 2, 2, 2, 3], [30, 1, 4, 6, 1]], dev)
+    axes = i32([i % 3 for i in range(D // 2)], dev)
+    inv = (1e6 ** (-torch.arange(D // 2, device=dev) / (D // 2))).float()
+    ntok, free = new(n), i32(np.random.default_rng(2).permutation(pool), dev)
+    count, zero = i32([pool], dev), new(n)
+    q, k, v = rows(Hq), rows(Hkv), rows(Hkv)
+
+    def buffers():
+        return dict(table=new(n, width), pos=new(T), slot=new(T), seq=new(T), cu=new(n + 1), limits=new(n), len=new(n),
+                    held=new(n), left=new(1), status=new(n), base=new(3), rope=new(3, T), q=rows(Hq), k=rows(Hkv),
+                    out=rows(Hq))
+
+    def step(b):
+        pkv.plan_step(zero, zero, ntok, b["table"], bs, pool, b["pos"], b["slot"], b["seq"], b["cu"], b["limits"], b["len"],
+                      b["held"], b["status"], free_list=free, free_count=count, free_count_out=b["left"])
+        pkv.rope_spans(scu, spans, b["base"])
+        pkv.rope_positions(b["pos"], b["seq"], scu, spans, b["base"], b["rope"])
+        pkv.rope_rows(q, k, b["rope"], axes, inv, b["q"], b["k"])
+        pkv.attn_packed(b["q"], b["k"], v, b["cu"], b["out"], D ** -0.5)
+
+    one, two = buffers(), buffers()
+    step(one)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        step(one)
+    for lens in ([100, 0, 250, 1, 49], [1, 1, 1, 1, 1], [400, 0, 0, 0, 0], [-20, 30, 60, -100, 8], [0, 0, 0, 0, 0]):
+        ntok.copy_(i32(lens, dev))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device=dev, generator=g))
+        for b in (one, two):
+            for x in b.values():
+                x.zero_()
+        graph.replay()
+        step(two)
+        torch.cuda.synchronize()
+        for name in one:
+            assert torch.equal(one[name], two[name]), (lens, name)
+        assert one["cu"].tolist() == np.concatenate([[0], np.cumsum(np.abs(lens))]).tolist()
+        used = int(one["cu"][-1])
+        assert (one["out"][used:] == 0).all() and (one["slot"][used:] == -1).all()

@@ -20,7 +20,7 @@ def packed(**kw):
     dict(T=-1), dict(seqs=-1), dict(Hq=0), dict(Hkv=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(cu=None), dict(cu=A + 2),
     dict(q=A + 8), dict(v=A + 2), dict(gate=A + 4), dict(q_row=-512), dict(k_row=100), dict(v_head=4), dict(o_row=32),
-    dict(o_head=32), dict(k_row=(1 << 24) + 8), dict(gate=A, g_row=3)])
+    dict(o_head=32), dict(o_row=64, o_head=64), dict(o_row=128, o_head=256), dict(k_row=(1 << 24) + 8), dict(gate=A, g_row=3)])
 def test_packed_refuses(kw):
     assert packed(**kw) == pkv.ERR_INVALID
 
@@ -79,7 +79,8 @@ def rope(**kw):
 @pytest.mark.parametrize("kw", [
     dict(T=-1), dict(Hq=-1), dict(Hkv=-1), dict(rot=-16), dict(stride=9), dict(q=None), dict(k=None), dict(qo=None),
     dict(ko=None), dict(rope=None), dict(axes=None), dict(inv=None), dict(q=A + 2), dict(ko=A + 8), dict(q_row=4),
-    dict(ko_head=-8), dict(qo_row=32), dict(ko_head=56), dict(qn=A + 2)])
+    dict(ko_head=-8), dict(qo_row=32), dict(ko_head=56), dict(qn=A + 2),
+    dict(qo_row=448), dict(ko_row=64)])
 def test_rope_rows_refuses(kw):
     assert rope(**kw) == pkv.ERR_INVALID
 
