@@ -25,7 +25,7 @@ def test_packed_refuses(kw):
     assert packed(**kw) == pkv.ERR_INVALID
 
 
-@pytest.mark.parametrize("kw", [dict(D=96), dict(D=0), dict(dtype=2), dict(Hq=7), dict(T=1 << 30, Hq=16, Hkv=2)])
+@pytest.mark.parametrize("kw", [dict(D=96), dict(D=0), dict(dtype=2), dict(Hq=7), dict(T=1 << 30, Hq=16, Hkv=2, o_row=1024)])
 def test_packed_does_not_serve(kw):
     assert packed(**kw) == pkv.ERR_UNSUPPORTED
 
