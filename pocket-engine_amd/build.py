@@ -1,7 +1,8 @@
 """Builds, in-tree next to the Python package that loads them:
 - libpkv.so: HIP kernels for gfx950 + the C-ABI + the host KV manager;
 - pkv_kernels.hsaco: the same kernel bodies under the reference engine's
-  kernel names and signatures (a code object for hipModuleLoadData)."""
+  kernel names and signatures (a code object for hipModuleLoadData);
+- _tensors.so: the Python package's checks of torch tensors (where torch is)."""
 import os
 import subprocess
 import sys
@@ -10,6 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "pkv", "libpkv.so")
 HSACO = os.path.join(HERE, "pkv", "pkv_kernels.hsaco")
+TENSORS = os.path.join(HERE, "pkv", "_tensors.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # Packed FP32 instructions are kept out of every code object.
@@ -37,10 +39,25 @@ def _run(cmd, what, verbose):
         raise RuntimeError(f"{what} build failed")
 
 
+def build_tensors(verbose=False):
+    """A plain C++ extension module: no device code, torch's headers only."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-I{root}/include",
+          "-I" + sysconfig.get_paths()["include"], f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          os.path.join(CSRC, "pkv_tensors.cpp"), f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", TENSORS],
+         "_tensors.so", verbose)
+
+
 def build(verbose=False):
     _run([HIPCC] + FLAGS + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", OUT], "libpkv.so", verbose)
     _run([HIPCC, "--genco"] + COMMON + [os.path.join(CSRC, "pkv_refabi.hip"), "-o", HSACO], "pkv_kernels.hsaco",
          verbose)
+    build_tensors(verbose)
     return OUT
 
 

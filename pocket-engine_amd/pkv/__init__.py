@@ -22,6 +22,11 @@ try:
     import torch
 except ImportError:
     torch = None
+if torch is not None:
+    # what the calls that take tensors ask of them; torch's libraries are loaded by now
+    if not os.path.exists(os.path.join(_HERE, "_tensors.so")):
+        raise ImportError(f"_tensors.so not built in {_HERE}: run __graft_entry__.build()")
+    from . import _tensors
 _lib = ctypes.CDLL(LIB_PATH)
 
 OK = 0
@@ -348,16 +353,23 @@ def attn_prefill_workspace(T, Hq, Hkv, seqs):
 # Calls that take whole tensors (shapes, strides and types from them). A tensor
 # of another shape or type than the call's, on the CPU, or on another device
 # than the others, raises PkvError(ERR_INVALID) before anything is launched;
-# the launch is on the tensors' device, whichever is current. (The checks are
-# written for their cost: a step's small calls are as long as their host time.)
+# the launch is on the tensors' device, whichever is current. The tensors are
+# looked at by _tensors, all arrays of a call at once.
 
 BF16, FP16 = 0, 1
+_I32, _F32 = 2, 3  # _tensors' types, beside those two
 
 
 def _refuse(what, why):
     e = PkvError(ERR_INVALID, what)
     e.args = (f"{what}: {why} ({ERR_INVALID})",)
     raise e
+
+
+def _wrong(what, names, wanted, r):
+    """_tensors' answer about an argument that will not do: 8 index + reason."""
+    name = names.split()[r // 8]
+    _refuse(what, f"{name} is on another device" if r % 8 == 3 else f"{name} is not {wanted}")
 
 
 def _launch(what, fn, dev, stream, *args):
@@ -377,33 +389,8 @@ def _launch(what, fn, dev, stream, *args):
         raise PkvError(status, what)
 
 
-def _words(what, dev, dtype, *arrays):
-    """The pointers of arrays (name, tensor, numel; None: any) of 32-bit words without gaps on device `dev`; None stays."""
-    out = []
-    for name, t, n in arrays:
-        if t is None:
-            out.append(None)
-            continue
-        if t.dtype is not dtype or (n is not None and t.numel() != n) or not t.is_contiguous():
-            _refuse(what, f"{name} is not a contiguous {dtype} array" + ("" if n is None else f" of {n}"))
-        if t.get_device() != dev:
-            _refuse(what, f"{name} is on another device")
-        out.append(t.data_ptr())
-    return out
-
-
-def _rows(what, dev, dtype, T, H, D, name, t):
-    """Pointer, row and head stride of [T, H, D] rows whose last dim has no gaps (a stride that nobody steps by is given
-    as a dense one)."""
-    if t.dtype is not dtype or t.dim() != 3:
-        _refuse(what, f"{name} is not [{T}, {H}, {D}] rows of {dtype}")
-    n, h, d = t.shape
-    row, head, one = t.stride()
-    if n != T or h != H or d != D or one != 1:
-        _refuse(what, f"{name} is not [{T}, {H}, {D}] rows of {dtype}, the last dim without gaps")
-    if t.get_device() != dev:
-        _refuse(what, f"{name} is on another device")
-    return t.data_ptr(), row if T > 1 else H * D, head if H > 1 else D
+_INTS = "a contiguous int32 tensor of the size that the call takes"
+_ROWS = "rows [T, heads, D] of q's T, D and type, the last dim without gaps"
 
 
 def _row_type(what, q, k):
@@ -411,9 +398,9 @@ def _row_type(what, q, k):
         _refuse(what, "q and k are not [T, heads, D]")
     dtype = q.dtype
     if dtype is torch.bfloat16:
-        return dtype, BF16
+        return BF16
     if dtype is torch.float16:
-        return dtype, FP16
+        return FP16
     raise PkvError(ERR_UNSUPPORTED, what)
 
 
@@ -429,12 +416,12 @@ def plan_step(len, held, ntok, block_table, block_size, num_blocks, pos, slot_ma
     T, dev = pos.numel(), pos.get_device()
     if free_list is not None and free_list.numel() < num_blocks:
         _refuse(what, "free_list holds fewer ids than the pool has pages")
-    (len, held, ntok, table, free_list, count, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out,
-     status) = _words(what, dev, torch.int32, ("len", len, n), ("held", held, n), ("ntok", ntok, n),
-                      ("block_table", block_table, None), ("free_list", free_list, None), ("free_count", free_count, 1),
-                      ("pos", pos, T), ("slot_map", slot_map, T), ("tok_seq", tok_seq, T), ("cu", cu, n + 1),
-                      ("limits", limits, n), ("len_out", len_out, n), ("held_out", held_out, n),
-                      ("free_count_out", free_count_out, 1), ("status", status, n))
+    r = _tensors.words(dev, _I32, len, n, held, n, ntok, n, block_table, -1, free_list, -1, free_count, 1, pos, T, slot_map, T,
+                       tok_seq, T, cu, n + 1, limits, n, len_out, n, held_out, n, free_count_out, 1, status, n)
+    if r.__class__ is int:
+        _wrong(what, "len held ntok block_table free_list free_count pos slot_map tok_seq cu limits len_out held_out "
+                     "free_count_out status", _INTS, r)
+    (len, held, ntok, table, free_list, count, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out, status) = r
     _launch(what, _lib.pkv_plan_step, dev, stream, len, held, ntok, n, table, width, block_size, num_blocks, free_list,
             count, T, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out, status)
 
@@ -448,9 +435,10 @@ def plan_truncate(new_len, len, held, block_table, block_size, num_blocks, free_
     dev = len.get_device()
     if free_list.numel() < num_blocks:
         _refuse(what, "free_list holds fewer ids than the pool has pages")
-    new_len, len, held, table, free_list, count = _words(
-        what, dev, torch.int32, ("new_len", new_len, n), ("len", len, n), ("held", held, n),
-        ("block_table", block_table, None), ("free_list", free_list, None), ("free_count", free_count, 1))
+    r = _tensors.words(dev, _I32, new_len, n, len, n, held, n, block_table, -1, free_list, -1, free_count, 1)
+    if r.__class__ is int:
+        _wrong(what, "new_len len held block_table free_list free_count", _INTS, r)
+    new_len, len, held, table, free_list, count = r
     _launch(what, _lib.pkv_plan_truncate, dev, stream, new_len, len, held, n, table, width, block_size, num_blocks,
             free_list, count)
 
@@ -462,20 +450,23 @@ def rope_spans(span_cu, spans, base, stream=None):
     n, dev, req = spans.shape[0], spans.get_device(), span_cu.numel() - 1
     if req < 0:
         _refuse(what, "span_cu is empty")
-    cu, spans, base = _words(what, dev, torch.int32, ("span_cu", span_cu, None), ("spans", spans, 5 * n), ("base", base, n))
-    _launch(what, _lib.pkv_rope_spans, dev, stream, cu, spans, req, n, base)
+    r = _tensors.words(dev, _I32, span_cu, -1, spans, 5 * n, base, n)
+    if r.__class__ is int:
+        _wrong(what, "span_cu spans base", _INTS, r)
+    _launch(what, _lib.pkv_rope_spans, dev, stream, r[0], r[1], req, n, r[2])
 
 
 def rope_positions(pos, tok_seq, span_cu, spans, base, rope, stream=None):
     """Time / height / width positions of a step's rows into rope [3, T] (or wider rows: rope[:, :T] is written)."""
     what = "pkv_rope_positions"
     T, n, dev, req = pos.numel(), spans.shape[0], pos.get_device(), span_cu.numel() - 1
-    if req < 0 or rope.dim() != 2 or rope.shape[0] != 3 or rope.shape[1] < T:
+    axes, stride = rope.shape if rope.dim() == 2 else (0, 0)
+    if req < 0 or axes != 3 or stride < T:
         _refuse(what, f"rope is not [3, {T} or more], or span_cu is empty")
-    stride = rope.shape[1]
-    pos, seq, cu, spans, base, rope = _words(
-        what, dev, torch.int32, ("pos", pos, T), ("tok_seq", tok_seq, T), ("span_cu", span_cu, None),
-        ("spans", spans, 5 * n), ("base", base, n), ("rope", rope, None))
+    r = _tensors.words(dev, _I32, pos, T, tok_seq, T, span_cu, -1, spans, 5 * n, base, n, rope, -1)
+    if r.__class__ is int:
+        _wrong(what, "pos tok_seq span_cu spans base rope", _INTS, r)
+    pos, seq, cu, spans, base, rope = r
     _launch(what, _lib.pkv_rope_positions, dev, stream, pos, seq, T, cu, spans, base, req, n, rope, stride)
 
 
@@ -483,33 +474,41 @@ def rope_rows(q, k, rope, axes, inv_freq, q_out, k_out, q_norm=None, k_norm=None
     """Norm (with weights) and rotation of q [T, Hq, D] and k [T, Hkv, D] rows into q_out and k_out (which may be q and
     k): rope [3, >= T] int32, axes [rot / 2] int32, inv_freq [rot / 2] f32 (see include/pkv.h)."""
     what = "pkv_rope_rows"
-    dtype, code = _row_type(what, q, k)
+    code = _row_type(what, q, k)
     T, Hq, D = q.shape
     Hkv, half, dev = k.shape[1], axes.numel(), q.get_device()
-    if rope.dim() != 2 or rope.shape[0] != 3 or rope.shape[1] < T:
+    n, stride = rope.shape if rope.dim() == 2 else (0, 0)
+    if n != 3 or stride < T:
         _refuse(what, f"rope is not [3, {T} or more]")
-    pos, ax = _words(what, dev, torch.int32, ("rope", rope, None), ("axes", axes, half))
-    inv, qn, kn = _words(what, dev, torch.float32, ("inv_freq", inv_freq, half), ("q_norm", q_norm, D), ("k_norm", k_norm, D))
-    _launch(what, _lib.pkv_rope_rows, dev, stream, *_rows(what, dev, dtype, T, Hq, D, "q", q),
-            *_rows(what, dev, dtype, T, Hkv, D, "k", k), *_rows(what, dev, dtype, T, Hq, D, "q_out", q_out),
-            *_rows(what, dev, dtype, T, Hkv, D, "k_out", k_out), Hq, Hkv, D, code, qn, kn, eps, pos, rope.shape[1], ax, inv,
-            2 * half, adjacent, T)
+    ints = _tensors.words(dev, _I32, rope, -1, axes, half)
+    if ints.__class__ is int:
+        _wrong(what, "rope axes", _INTS, ints)
+    floats = _tensors.words(dev, _F32, inv_freq, half, q_norm, D, k_norm, D)
+    if floats.__class__ is int:
+        _wrong(what, "inv_freq q_norm k_norm", "a contiguous float32 tensor of the size that the call takes", floats)
+    rows = _tensors.rows(dev, code, T, D, q, Hq, k, Hkv, q_out, Hq, k_out, Hkv)
+    if rows.__class__ is int:
+        _wrong(what, "q k q_out k_out", _ROWS, rows)
+    _launch(what, _lib.pkv_rope_rows, dev, stream, *rows, Hq, Hkv, D, code, floats[1], floats[2], eps, ints[0], stride,
+            ints[1], floats[0], 2 * half, adjacent, T)
 
 
 def attn_packed(q, k, v, cu, out, scale, gate=None, stream=None):
     """Causal attention over packed whole prompts, no cache (see include/pkv.h): q, out (and gate) [T, Hq, D], k and v
     [T, Hkv, D] of bfloat16 or float16, any row and head strides; cu [sequences + 1] int32."""
     what = "pkv_attn_packed"
-    dtype, code = _row_type(what, q, k)
+    code = _row_type(what, q, k)
     T, Hq, D = q.shape
     Hkv, dev, seqs = k.shape[1], q.get_device(), cu.numel() - 1
     if seqs < 0:
         _refuse(what, "cu is empty")
-    (offsets,) = _words(what, dev, torch.int32, ("cu", cu, None))
-    _launch(what, _lib.pkv_attn_packed, dev, stream, *_rows(what, dev, dtype, T, Hq, D, "q", q),
-            *_rows(what, dev, dtype, T, Hkv, D, "k", k), *_rows(what, dev, dtype, T, Hkv, D, "v", v),
-            *((None, 0, 0) if gate is None else _rows(what, dev, dtype, T, Hq, D, "gate", gate)),
-            *_rows(what, dev, dtype, T, Hq, D, "out", out), offsets, seqs, T, Hq, Hkv, D, code, scale)
+    offsets = _tensors.words(dev, _I32, cu, -1)
+    if offsets.__class__ is int:
+        _wrong(what, "cu", _INTS, offsets)
+    rows = _tensors.rows(dev, code, T, D, q, Hq, k, Hkv, v, Hkv, gate, Hq, out, Hq)
+    if rows.__class__ is int:
+        _wrong(what, "q k v gate out", _ROWS, rows)
+    _launch(what, _lib.pkv_attn_packed, dev, stream, *rows, offsets[0], seqs, T, Hq, Hkv, D, code, scale)
 
 
 class Pool:
