@@ -2,7 +2,7 @@
 - libpkv.so: HIP kernels for gfx950 + the C-ABI + the host KV manager;
 - pkv_kernels.hsaco: the same kernel bodies under the reference engine's
   kernel names and signatures (a code object for hipModuleLoadData);
-- _tensors.so: the Python package's checks of torch tensors (where torch is)."""
+- _tensors.so: the Python package's calls that take torch tensors (where torch is)."""
 import os
 import subprocess
 import sys
@@ -49,7 +49,7 @@ def build_tensors(verbose=False):
     root = os.path.dirname(os.path.abspath(torch.__file__))
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-I{root}/include",
           "-I" + sysconfig.get_paths()["include"], f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          os.path.join(CSRC, "pkv_tensors.cpp"), f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", TENSORS],
+          os.path.join(CSRC, "pkv_tensors.cpp"), f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl", "-o", TENSORS],
          "_tensors.so", verbose)
 
 

@@ -23,11 +23,13 @@ try:
 except ImportError:
     torch = None
 if torch is not None:
-    # what the calls that take tensors ask of them; torch's libraries are loaded by now
+    # the calls that take whole tensors; torch's libraries are loaded by now
     if not os.path.exists(os.path.join(_HERE, "_tensors.so")):
         raise ImportError(f"_tensors.so not built in {_HERE}: run __graft_entry__.build()")
     from . import _tensors
 _lib = ctypes.CDLL(LIB_PATH)
+if torch is not None:
+    _tensors.bind(LIB_PATH)
 
 OK = 0
 ERR_INVALID = 1
@@ -353,162 +355,108 @@ def attn_prefill_workspace(T, Hq, Hkv, seqs):
 # Calls that take whole tensors (shapes, strides and types from them). A tensor
 # of another shape or type than the call's, on the CPU, or on another device
 # than the others, raises PkvError(ERR_INVALID) before anything is launched;
-# the launch is on the tensors' device, whichever is current. The tensors are
-# looked at by _tensors, all arrays of a call at once.
-
-BF16, FP16 = 0, 1
-_I32, _F32 = 2, 3  # _tensors' types, beside those two
+# the launch is on the tensors' device, whichever is current.
 
 
-def _refuse(what, why):
-    e = PkvError(ERR_INVALID, what)
-    e.args = (f"{what}: {why} ({ERR_INVALID})",)
-    raise e
-
-
-def _wrong(what, names, wanted, r):
-    """_tensors' answer about an argument that will not do: 8 index + reason."""
-    name = names.split()[r // 8]
-    _refuse(what, f"{name} is on another device" if r % 8 == 3 else f"{name} is not {wanted}")
-
-
-def _launch(what, fn, dev, stream, *args):
-    """fn(*args, stream) on device `dev`, stream None: torch's current one there."""
-    if dev < 0:
-        _refuse(what, "the tensors are not on a GPU")
+def _raw_stream(stream, dev):
+    """A stream's handle; None: torch's current one on device `dev`."""
     if stream is None:
-        stream = torch._C._cuda_getCurrentRawStream(dev)
-    elif not isinstance(stream, int):
-        stream = stream.cuda_stream
-    if dev == torch._C._cuda_getDevice():
-        status = fn(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, stream)
-    if status != OK:
-        raise PkvError(status, what)
+        return torch._C._cuda_getCurrentRawStream(dev) if dev >= 0 else 0
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-_INTS = "a contiguous int32 tensor of the size that the call takes"
-_ROWS = "rows [T, heads, D] of q's T, D and type, the last dim without gaps"
+def _elsewhere(dev):
+    """Whether `dev` is a GPU and not the current one."""
+    return dev >= 0 and dev != torch._C._cuda_getDevice()
 
 
-def _row_type(what, q, k):
-    if q.dim() != 3 or k.dim() != 3:
-        _refuse(what, "q and k are not [T, heads, D]")
-    dtype = q.dtype
-    if dtype is torch.bfloat16:
-        return BF16
-    if dtype is torch.float16:
-        return FP16
-    raise PkvError(ERR_UNSUPPORTED, what)
+def _failed(what, r, names):
+    """Raises for _tensors' answer r: a status, or below 0 what is wrong with which of the named tensors."""
+    if r > 0:
+        raise PkvError(r, what)
+    name = names.split()[-r // 8]
+    why = ("", "is not a tensor", "is not of the type, sizes and strides that the call takes",
+           "is on another device than the others", "is not on a GPU")[-r % 8]
+    e = PkvError(ERR_INVALID, what)
+    e.args = (f"{what}: {name} {why} ({ERR_INVALID})",)
+    raise e
 
 
 def plan_step(len, held, ntok, block_table, block_size, num_blocks, pos, slot_map, tok_seq, cu, limits, len_out, held_out,
               status, free_list=None, free_count=None, free_count_out=None, stream=None):
     """A step's pages, slots and row metadata from the requests' lengths, on
     the GPU (see include/pkv.h): block_table [rows, max_blocks], pos / slot_map
-    / tok_seq [T], all int32."""
-    what = "pkv_plan_step"
-    if block_table.dim() != 2:
-        _refuse(what, "block_table is not [rows, max_blocks]")
-    n, width = block_table.shape
-    T, dev = pos.numel(), pos.get_device()
-    if free_list is not None and free_list.numel() < num_blocks:
-        _refuse(what, "free_list holds fewer ids than the pool has pages")
-    r = _tensors.words(dev, _I32, len, n, held, n, ntok, n, block_table, -1, free_list, -1, free_count, 1, pos, T, slot_map, T,
-                       tok_seq, T, cu, n + 1, limits, n, len_out, n, held_out, n, free_count_out, 1, status, n)
-    if r.__class__ is int:
-        _wrong(what, "len held ntok block_table free_list free_count pos slot_map tok_seq cu limits len_out held_out "
-                     "free_count_out status", _INTS, r)
-    (len, held, ntok, table, free_list, count, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out, status) = r
-    _launch(what, _lib.pkv_plan_step, dev, stream, len, held, ntok, n, table, width, block_size, num_blocks, free_list,
-            count, T, pos, slot_map, tok_seq, cu, limits, len_out, held_out, count_out, status)
+    / tok_seq [T], free_list [num_blocks or more], all int32 without gaps."""
+    dev = block_table.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return plan_step(len, held, ntok, block_table, block_size, num_blocks, pos, slot_map, tok_seq, cu, limits,
+                             len_out, held_out, status, free_list, free_count, free_count_out, stream)
+    r = _tensors.plan_step(dev, _raw_stream(stream, dev), block_table, pos, len, held, ntok, slot_map, tok_seq, cu, limits,
+                           len_out, held_out, status, free_list, free_count, free_count_out, block_size, num_blocks)
+    if r:
+        _failed("pkv_plan_step", r, "block_table pos len held ntok slot_map tok_seq cu limits len_out held_out status "
+                                    "free_list free_count free_count_out")
 
 
 def plan_truncate(new_len, len, held, block_table, block_size, num_blocks, free_list, free_count, stream=None):
     """Rows cut to new_len positions, their pages back to the free list (see include/pkv.h)."""
-    what = "pkv_plan_truncate"
-    if block_table.dim() != 2:
-        _refuse(what, "block_table is not [rows, max_blocks]")
-    n, width = block_table.shape
-    dev = len.get_device()
-    if free_list.numel() < num_blocks:
-        _refuse(what, "free_list holds fewer ids than the pool has pages")
-    r = _tensors.words(dev, _I32, new_len, n, len, n, held, n, block_table, -1, free_list, -1, free_count, 1)
-    if r.__class__ is int:
-        _wrong(what, "new_len len held block_table free_list free_count", _INTS, r)
-    new_len, len, held, table, free_list, count = r
-    _launch(what, _lib.pkv_plan_truncate, dev, stream, new_len, len, held, n, table, width, block_size, num_blocks,
-            free_list, count)
+    dev = block_table.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return plan_truncate(new_len, len, held, block_table, block_size, num_blocks, free_list, free_count, stream)
+    r = _tensors.plan_truncate(dev, _raw_stream(stream, dev), block_table, new_len, len, held, free_list, free_count,
+                               block_size, num_blocks)
+    if r:
+        _failed("pkv_plan_truncate", r, "block_table new_len len held free_list free_count")
 
 
 def rope_spans(span_cu, spans, base, stream=None):
     """The position at which each media span of each request starts (see include/pkv.h): spans [n, 5] int32 rows
     (start, t, h, w, step), span_cu [requests + 1], base [n]."""
-    what = "pkv_rope_spans"
-    n, dev, req = spans.shape[0], spans.get_device(), span_cu.numel() - 1
-    if req < 0:
-        _refuse(what, "span_cu is empty")
-    r = _tensors.words(dev, _I32, span_cu, -1, spans, 5 * n, base, n)
-    if r.__class__ is int:
-        _wrong(what, "span_cu spans base", _INTS, r)
-    _launch(what, _lib.pkv_rope_spans, dev, stream, r[0], r[1], req, n, r[2])
+    dev = spans.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_spans(span_cu, spans, base, stream)
+    r = _tensors.rope_spans(dev, _raw_stream(stream, dev), span_cu, spans, base)
+    if r:
+        _failed("pkv_rope_spans", r, "span_cu spans base")
 
 
 def rope_positions(pos, tok_seq, span_cu, spans, base, rope, stream=None):
     """Time / height / width positions of a step's rows into rope [3, T] (or wider rows: rope[:, :T] is written)."""
-    what = "pkv_rope_positions"
-    T, n, dev, req = pos.numel(), spans.shape[0], pos.get_device(), span_cu.numel() - 1
-    axes, stride = rope.shape if rope.dim() == 2 else (0, 0)
-    if req < 0 or axes != 3 or stride < T:
-        _refuse(what, f"rope is not [3, {T} or more], or span_cu is empty")
-    r = _tensors.words(dev, _I32, pos, T, tok_seq, T, span_cu, -1, spans, 5 * n, base, n, rope, -1)
-    if r.__class__ is int:
-        _wrong(what, "pos tok_seq span_cu spans base rope", _INTS, r)
-    pos, seq, cu, spans, base, rope = r
-    _launch(what, _lib.pkv_rope_positions, dev, stream, pos, seq, T, cu, spans, base, req, n, rope, stride)
+    dev = pos.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_positions(pos, tok_seq, span_cu, spans, base, rope, stream)
+    r = _tensors.rope_positions(dev, _raw_stream(stream, dev), span_cu, spans, base, pos, tok_seq, rope)
+    if r:
+        _failed("pkv_rope_positions", r, "span_cu spans base pos tok_seq rope")
 
 
 def rope_rows(q, k, rope, axes, inv_freq, q_out, k_out, q_norm=None, k_norm=None, eps=1e-6, adjacent=False, stream=None):
     """Norm (with weights) and rotation of q [T, Hq, D] and k [T, Hkv, D] rows into q_out and k_out (which may be q and
     k): rope [3, >= T] int32, axes [rot / 2] int32, inv_freq [rot / 2] f32 (see include/pkv.h)."""
-    what = "pkv_rope_rows"
-    code = _row_type(what, q, k)
-    T, Hq, D = q.shape
-    Hkv, half, dev = k.shape[1], axes.numel(), q.get_device()
-    n, stride = rope.shape if rope.dim() == 2 else (0, 0)
-    if n != 3 or stride < T:
-        _refuse(what, f"rope is not [3, {T} or more]")
-    ints = _tensors.words(dev, _I32, rope, -1, axes, half)
-    if ints.__class__ is int:
-        _wrong(what, "rope axes", _INTS, ints)
-    floats = _tensors.words(dev, _F32, inv_freq, half, q_norm, D, k_norm, D)
-    if floats.__class__ is int:
-        _wrong(what, "inv_freq q_norm k_norm", "a contiguous float32 tensor of the size that the call takes", floats)
-    rows = _tensors.rows(dev, code, T, D, q, Hq, k, Hkv, q_out, Hq, k_out, Hkv)
-    if rows.__class__ is int:
-        _wrong(what, "q k q_out k_out", _ROWS, rows)
-    _launch(what, _lib.pkv_rope_rows, dev, stream, *rows, Hq, Hkv, D, code, floats[1], floats[2], eps, ints[0], stride,
-            ints[1], floats[0], 2 * half, adjacent, T)
+    dev = q.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_rows(q, k, rope, axes, inv_freq, q_out, k_out, q_norm, k_norm, eps, adjacent, stream)
+    r = _tensors.rope_rows(dev, _raw_stream(stream, dev), q, k, q_out, k_out, rope, axes, inv_freq, q_norm, k_norm, eps,
+                           adjacent)
+    if r:
+        _failed("pkv_rope_rows", r, "q k q_out k_out rope axes inv_freq q_norm k_norm")
 
 
 def attn_packed(q, k, v, cu, out, scale, gate=None, stream=None):
     """Causal attention over packed whole prompts, no cache (see include/pkv.h): q, out (and gate) [T, Hq, D], k and v
     [T, Hkv, D] of bfloat16 or float16, any row and head strides; cu [sequences + 1] int32."""
-    what = "pkv_attn_packed"
-    code = _row_type(what, q, k)
-    T, Hq, D = q.shape
-    Hkv, dev, seqs = k.shape[1], q.get_device(), cu.numel() - 1
-    if seqs < 0:
-        _refuse(what, "cu is empty")
-    offsets = _tensors.words(dev, _I32, cu, -1)
-    if offsets.__class__ is int:
-        _wrong(what, "cu", _INTS, offsets)
-    rows = _tensors.rows(dev, code, T, D, q, Hq, k, Hkv, v, Hkv, gate, Hq, out, Hq)
-    if rows.__class__ is int:
-        _wrong(what, "q k v gate out", _ROWS, rows)
-    _launch(what, _lib.pkv_attn_packed, dev, stream, *rows, offsets[0], seqs, T, Hq, Hkv, D, code, scale)
+    dev = q.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return attn_packed(q, k, v, cu, out, scale, gate, stream)
+    r = _tensors.attn_packed(dev, _raw_stream(stream, dev), q, k, v, out, gate, cu, scale)
+    if r:
+        _failed("pkv_attn_packed", r, "q k v out gate cu")
 
 
 class Pool:

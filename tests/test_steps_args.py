@@ -113,7 +113,7 @@ def test_python_forms_check_their_tensors():
     I, U = pkv.ERR_INVALID, pkv.ERR_UNSUPPORTED
     q, k, cu = bf(6, 4, 64), bf(6, 2, 64), i32(3)
     f = pkv.attn_packed
-    assert "are not on a GPU" in raises(I, f, q, k, k, cu, q, 0.1)
+    assert "not on a GPU" in raises(I, f, q, k, k, cu, q, 0.1)
     raises(U, f, q.float(), k.float(), k.float(), cu, q.float(), 0.1)
     raises(I, f, q, k.half(), k, cu, q, 0.1)
     raises(I, f, q, k, k[:5], cu, q, 0.1)
@@ -126,7 +126,7 @@ def test_python_forms_check_their_tensors():
     raises(I, f, q[0], k, k, cu, q, 0.1)
     rope, axes, inv = i32(3, 6), i32(16), torch.zeros(16)
     f = pkv.rope_rows
-    assert "are not on a GPU" in raises(I, f, q, k, rope, axes, inv, q, k)
+    assert "not on a GPU" in raises(I, f, q, k, rope, axes, inv, q, k)
     raises(I, f, q, k, i32(3, 5), axes, inv, q, k)
     raises(I, f, q, k, i32(2, 6), axes, inv, q, k)
     raises(I, f, q, k, rope, axes, inv[:8], q, k)
@@ -134,12 +134,12 @@ def test_python_forms_check_their_tensors():
     raises(I, f, q, k, rope, axes, inv, q, k, q_norm=torch.zeros(32))
     raises(I, f, q, k, rope, axes, inv, q[:5], k)
     spans, scu, base = i32(4, 5), i32(3), i32(4)
-    assert "are not on a GPU" in raises(I, pkv.rope_spans, scu, spans, base)
+    assert "not on a GPU" in raises(I, pkv.rope_spans, scu, spans, base)
     raises(I, pkv.rope_spans, scu, i32(4, 4), base)
     raises(I, pkv.rope_spans, i32(0), spans, base)
     raises(I, pkv.rope_spans, scu, spans, i32(3))
     pos = i32(6)
-    assert "are not on a GPU" in raises(I, pkv.rope_positions, pos, pos, scu, spans, base, rope)
+    assert "not on a GPU" in raises(I, pkv.rope_positions, pos, pos, scu, spans, base, rope)
     raises(I, pkv.rope_positions, pos, i32(5), scu, spans, base, rope)
     raises(I, pkv.rope_positions, pos, pos, scu, spans, base, i32(3, 5))
     raises(I, pkv.rope_positions, pos, pos, scu, spans, i32(2), rope)
@@ -147,12 +147,12 @@ def test_python_forms_check_their_tensors():
     step = lambda **kw: pkv.plan_step(**{**dict(len=r3, held=r3, ntok=r3, block_table=table, block_size=16, num_blocks=8,
                                                 pos=t, slot_map=t, tok_seq=t, cu=i32(4), limits=r3, len_out=r3, held_out=r3,
                                                 status=r3, free_list=i32(8), free_count=i32(1)), **kw})
-    assert "are not on a GPU" in raises(I, step)
+    assert "not on a GPU" in raises(I, step)
     for kw in (dict(len=i32(2)), dict(cu=r3), dict(block_table=i32(12)), dict(slot_map=i32(8)), dict(free_list=i32(7)),
                dict(free_count=i32(2)), dict(status=r3.long()), dict(block_table=i32(4, 3).t())):
         raises(I, lambda: step(**kw))
     cut = lambda **kw: pkv.plan_truncate(**{**dict(new_len=r3, len=r3, held=r3, block_table=table, block_size=16,
                                                    num_blocks=8, free_list=i32(8), free_count=i32(1)), **kw})
-    assert "are not on a GPU" in raises(I, cut)
+    assert "not on a GPU" in raises(I, cut)
     for kw in (dict(new_len=i32(2)), dict(free_list=i32(7)), dict(free_count=r3), dict(block_table=i32(12))):
         raises(I, lambda: cut(**kw))
