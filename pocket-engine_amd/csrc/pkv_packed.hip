@@ -278,6 +278,25 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++) qf[kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
     }
+    // The gates of the rows that a lane writes at the end (pass ps, row k). With
+    // several key groups they are few enough to be requested here (at 256 dims
+    // they would push the sums out of the first 256 registers); else they come
+    // before the first output pass.
+    constexpr int PW = S::PW, RPI = S::RPI, RK = 32 / (RPI * KS);  // RK rows a lane
+    const int er = lane / S::LPR, ec = lane % S::LPR;
+    uint4 gr[D / PW][RK];
+    auto load_gates = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < RK; k++) {
+            int qq, hh;
+            split(wrow + RPI * (RK * kg + k) + er, qq, hh);
+            const uint16_t* src = p.gate + (size_t)(c0 + qq) * p.g_row + (size_t)(kvh * p.G + hh) * p.g_head + 8 * ec;
+#pragma unroll
+            for (int ps = 0; ps < D / PW; ps++) gr[ps][k] = *reinterpret_cast<const uint4*>(src + PW * ps);
+        }
+    };
+    constexpr bool EARLY = KS > 1 && D < 256;
+    if (EARLY && p.gate) load_gates();
     f32x16 o[D / 32];
     // running maximum (log2 units; 0 before the first key; may lag, below) and
     // the lane's own part of the sum
@@ -378,31 +397,55 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     // it, so those two say what the finished rows get.
     auto tame = [&](int k0, int buf) __attribute__((always_inline)) {
         if (k0 + BK - 1 <= first_q) return;
+        uint4* at = reinterpret_cast<uint4*>(stage + buf * S::STAGE + NG * S::KG + g0 * S::VG + 16 * lane);
+        bool bad = false;
+        if constexpr (D == 256 && KS == 1) {
+            // (4 groups. Looked at together as below they leave the loop's
+            // registers 2 % slower: one prompt of 4,096 tokens at 24 / 4 heads
+            // 212 -> 216 us.)
+            auto odd_pair = [](uint32_t w) {  // a half whose exponent is all ones
+                const uint32_t u = ~w & E::EXP;
+                return (u & 0xffffu) == 0 || u < 0x10000u;
+            };
 #pragma unroll
-        for (int i = 0; i < S::PER; i++) {
-            uint4* at = reinterpret_cast<uint4*>(stage + buf * S::STAGE + NG * S::KG + (g0 + i) * S::VG + 16 * lane);
-            const uint4 x = *at;
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t u = ~w[e] & E::EXP;  // a half of 0: not finite
-                bad |= (u & 0xffffu) == 0 || (u >> 16) == 0;
+            for (int i = 0; i < S::PER; i++) {
+                const uint4 x = at[i * (S::VG / 16)];
+                bad |= odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
             }
-            if (bad) {
-                const int key = k0 + g0 + i + NG * lb;
+        } else {
+            // All the wave's groups are read before one is looked at: by the
+            // largest exponent bits of either half (a wave with 16 groups
+            // 4,400 -> 900 cycles; one prompt of 37 tokens 9.7 -> 8.2 us).
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < S::PER; i++) {
+                const uint4 x = at[i * (S::VG / 16)];
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[e] & E::EXP));
+            }
+            const unsigned short all = (unsigned short)E::EXP;
+            bad = top.x == all || top.y == all;
+        }
+        if (!__any(bad)) return;
 #pragma unroll 1
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t y = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-                    if ((~y & E::EXP & 0xffffu) != 0) continue;
-                    const bool nan = y & E::MANT & 0xffffu, minus = y >> 15;
-                    if (nan || !minus) atomicMin(odd + 8 * lc + e, key);
-                    if (nan || minus) atomicMin(odd + D + 8 * lc + e, key);
-                    w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
-                }
-                *at = make_uint4(w[0], w[1], w[2], w[3]);
-                odd[2 * D] = 1;
+        for (int i = 0; i < S::PER; i++) {
+            if (!bad) continue;
+            const uint4 x = at[i * (S::VG / 16)];
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            const int key = k0 + g0 + i + NG * lb;
+#pragma unroll 1
+            for (int e = 0; e < 8; e++) {
+                const uint32_t y = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                if ((~y & E::EXP & 0xffffu) != 0) continue;
+                const bool nan = y & E::MANT & 0xffffu, minus = y >> 15;
+                if (nan || !minus) atomicMin(odd + 8 * lc + e, key);
+                if (nan || minus) atomicMin(odd + D + 8 * lc + e, key);
+                w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
             }
+            at[i * (S::VG / 16)] = make_uint4(w[0], w[1], w[2], w[3]);
+            odd[2 * D] = 1;
         }
     };
 
@@ -445,7 +488,6 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     // gate), and leave as 16-byte pieces, LPR lanes per row. With several key
     // groups their sums, brought to the same maximum, are added there, each
     // group's wave finishing its part of the 32 rows.
-    constexpr int PW = S::PW, RPI = S::RPI, RK = 32 / (RPI * KS);  // RK rows a lane
     __shared__ float join[KS > 1 ? NW : 1][2][32];
     if constexpr (KS > 1) {
         l = add_xor32(l);
@@ -456,30 +498,20 @@ __device__ __forceinline__ void packed_tile(const PackedParams& p, char* smem, i
     }
     __syncthreads();  // every wave is past the last tile's stage
     float* const out_stage = reinterpret_cast<float*>(smem) + rg * 32 * S::RR;  // key group g's: + g RG 32 RR
-    const int er = lane / S::LPR, ec = lane % S::LPR;
     const bool any_odd = odd[2 * D] != 0;
     size_t t[RK];
     int head[RK], query[RK];
     bool ok[RK];
 #pragma unroll
     for (int k = 0; k < RK; k++) {
-        const int r = wrow + RPI * RK * kg + er + RPI * k;
+        const int r = wrow + RPI * (RK * kg + k) + er;
         int hh;
         split(r, query[k], hh);
         ok[k] = r < rows;
         t[k] = (size_t)(c0 + query[k]);
         head[k] = kvh * p.G + hh;
     }
-    // every pass's gates, requested before the first pass
-    uint4 gr[D / PW][RK];
-    if (p.gate) {
-#pragma unroll
-        for (int ps = 0; ps < D / PW; ps++)
-#pragma unroll
-            for (int k = 0; k < RK; k++)
-                gr[ps][k] = *reinterpret_cast<const uint4*>(p.gate + t[k] * p.g_row + (size_t)head[k] * p.g_head + PW * ps +
-                                                            8 * ec);
-    }
+    if (!EARLY && p.gate) load_gates();
     float inv;
     if constexpr (KS > 1) {
         float top = -INFINITY, sum = 0.f;
