@@ -27,11 +27,11 @@ int launch(const pkv::PackedParams& p, hipStream_t stream) {
 // mean length n = T / seqs, and the grid takes the longest workgroup or, where
 // it holds more than the card's places, the places' turns at the mean (half the
 // keys, causal). Measured, us, for 1 x 4, 2 x 2 and 4 x 1 (RG x KS): 256 dims at
-// 16 / 4 heads, one prompt of 600 tokens 22 / 25 / 31, 1,200 47 / 39 / 52, 2,400
-// 118 / 104 / 96, 20 of 60 31 / 23 / 14; 128 dims at 32 / 8, 500 11 / 13 / 17,
-// 1,200 33 / 25 / 33, 16 of 200 49 / 32 / 22; 64 dims at 12 / 2, 2,000 18 / 22 /
-// 38, 4,000 48 / 45 / 73. The estimate takes the fastest, or one within 16 %, in
-// all 29 batches that were timed.
+// 16 / 4 heads, one prompt of 600 tokens 18 / 22 / 31, 1,200 39 / 35 / 51, 2,400
+// 100 / 91 / 95, 20 of 60 26 / 21 / 14; 128 dims at 32 / 8, 500 10 / 11 / 16,
+// 1,200 29 / 23 / 32, 16 of 200 44 / 29 / 21; 64 dims at 12 / 2, 2,000 16 / 22 /
+// 37, 4,000 44 / 44 / 70. The estimate takes the fastest, or one within 10 %, in
+// all 35 batches that were timed.
 struct Shape {
     int rows, ks, places;  // rows of a workgroup, key groups, workgroups a CU holds
 };
