@@ -363,8 +363,8 @@ int pkv_attn_prefill_e4m3_split(const void* q, const void* kcache, const void* v
  * have pos = k and slot -1, tokens past the last row up to T have pos 0, slot
  * -1 and tok_seq 0, so that a step captured for T tokens never stores them.
  * limits[s] = pages * block_size - 1 (-1 for padding rows and rows with a
- * status). len_out, held_out, free_count_out (may be null): the state after
- * the step; each may be its input. status[s]: 0; PKV_ERR_NO_BLOCKS where the
+ * status). len_out, held_out and free_count_out (the last may be null): the
+ * state after the step; each may be its input. status[s]: 0; PKV_ERR_NO_BLOCKS where the
  * free pages do not cover the row and the rows before it that need pages (it
  * takes none, nor do later rows that need some); PKV_ERR_INVALID where its
  * lengths do not fit its table (or, without a free list, its pages), or its
@@ -421,11 +421,12 @@ int pkv_rope_positions(const int32_t* pos, const int32_t* tok_seq, int T, const 
  * for pair i < rot / 2 of the first rot dims, (a, b) = (i, i + rot / 2), or
  * (2 i, 2 i + 1) with adjacent; dims from rot on are y. axes[i] (int32) is the
  * axis of pair i (values other than 1 and 2: time), so any sections of axes,
- * one after the other or interleaved. Angles are exact to 2^-40 of a turn at
- * any position, the arithmetic is f32, rounded once at the end (pkv_attn_prep
- * rounds where the reference does). Rows and strides as pkv_attn_packed; each
- * out may be its input (same strides), else they may not overlap. rot is a multiple of 16
- * (0: norm alone). Hq or Hkv may be 0. */
+ * one after the other or interleaved. Angles come from 64 bits (within 2^-51
+ * of their size: 2^-34 of a turn at position 2^20), the rest of the arithmetic
+ * is f32, rounded once at the end (pkv_attn_prep rounds where the reference
+ * does). Rows and strides as pkv_attn_packed; each out may be its input (same
+ * strides), else they may not overlap. rot is a multiple of 16 (0: norm alone).
+ * Hq or Hkv may be 0. */
 int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                   void* q_out, int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row,
                   int64_t k_out_head, int Hq, int Hkv, int D, int dtype, const float* q_norm, const float* k_norm,
