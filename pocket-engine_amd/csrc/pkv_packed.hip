@@ -151,6 +151,7 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
         const int incl = wave_prefix(k);
         int r = tile - after - (incl - k), a = 0, b = 0;
         const unsigned long long hit = __ballot(r >= 0 && r < k);
+        if (hit == 0) return false;  // offsets that decrease, with counts past 31 bits
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (c[i] > lo && r-- == 0) {
@@ -175,6 +176,7 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
     }
     const int incl = wave_prefix(sum);
     if (lane == 63) wsum[wave] = incl;
+    if (tid < 3) found[tid] = 0;
     __syncthreads();
     int total = 0, before = 0;
 #pragma unroll
@@ -203,7 +205,7 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
     c0 = __builtin_amdgcn_readfirstlane(found[0]);
     n = __builtin_amdgcn_readfirstlane(found[1]);
     x = __builtin_amdgcn_readfirstlane(found[2]);
-    return true;
+    return n > 0;  // (0: offsets that decrease, with counts past 31 bits)
 }
 
 // s_waitcnt lgkmcnt(0) that leaves the other counters alone, and keeps memory

@@ -43,7 +43,7 @@ void launch_rope(const pkv::RopeParams& p, hipStream_t stream) {
     // loses more than the writer gains: 4,096 rows 44.5 -> 45.5 us with theirs.
     const bool large = (int64_t)p.T * (p.Hq + p.Hkv) * D * 2 > 160000000;
     const auto kernel = large ? pkv::rope_rows_kernel<E, D, ADJ, true> : pkv::rope_rows_kernel<E, D, ADJ, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.T + tb - 1) / tb)), dim3(256), 0, stream, p, tb);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.T - 1) / tb + 1)), dim3(256), 0, stream, p, tb);
 }
 template <class E, bool ADJ>
 void rope_by_dims(const pkv::RopeParams& p, int D, hipStream_t stream) {
@@ -127,7 +127,7 @@ int pkv_rope_positions(const int32_t* pos, const int32_t* tok_seq, int T, const 
     if (T == 0) return PKV_OK;
     if (!words({pos, tok_seq, rope}) || (n_req > 0 && !words({span_cu})) || (n_spans > 0 && !words({spans, base})))
         return PKV_ERR_INVALID;
-    hipLaunchKernelGGL(pkv::rope_positions_kernel, dim3((T + 255) / 256), dim3(256), 0, (hipStream_t)stream, pos, tok_seq,
+    hipLaunchKernelGGL(pkv::rope_positions_kernel, dim3((T - 1) / 256 + 1), dim3(256), 0, (hipStream_t)stream, pos, tok_seq,
                        span_cu, spans, base, n_req, n_spans, T, rope, rope_stride);
     return launch_status();
 }
