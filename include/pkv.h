@@ -457,7 +457,8 @@ int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, i
  * reaches exactly the rows that attend it. The same call gives the same bits;
  * how a batch's keys are shared out, and with it the last bits of a row, goes
  * by T, seqs and the heads. scale is finite and above 0. PKV_ERR_UNSUPPORTED
- * for other types, dims or groups, or T G above 2^30. No workspace. No
+ * for other types, dims or groups, T G above 2^30, or sequences times kv heads
+ * of 2^24 or more. No workspace. No
  * reference counterpart (the reference attends through its pages only,
  * src/model.rs:2438-2493). */
 int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,

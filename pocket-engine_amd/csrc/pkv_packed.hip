@@ -50,6 +50,7 @@ struct PackedParams {
     int seqs, T, Hkv, G;
     uint32_t g_mul;  // query of a row: its number divided by G (div_group)
     int g_shift;
+    int band_shift;  // find_packed_tile
     float scale2;  // scale * log2(e)
 };
 
@@ -94,19 +95,29 @@ struct PackedTile {
 };
 
 // This workgroup's sequence (rows c0 .. c0 + n - 1) and its tile x of it. False
-// where the grid has more workgroups than the batch has tiles. A tile x of any
-// sequence attends up to (x + 1) RW / G keys, so the order of the tiles is the
-// order of their work, and the longest are started first, whatever the
-// sequences' order (LEVEL_SEQS sequences or fewer): with c_s tiles in sequence
-// s, N(j) = sum_s max(0, c_s - j) tiles have x >= j, so the tile of rank r has
-// the largest x with N(x) > r, found by halving. Every wave does it for
-// itself, 4 sequences to a lane, without LDS or barriers (about 0.5 us beside
-// the offsets' load). More sequences: last sequence first, the tiles of each
-// from the last, by a prefix sum over the workgroup's threads.
+// where the grid has more workgroups than the batch has tiles. Every wave finds
+// them for itself, without LDS or barriers.
+//
+// LEVEL_SEQS sequences or fewer: a tile x of any sequence attends up to (x + 1)
+// RW / G keys, so the order of the tiles is the order of their work, and the
+// longest are started first, whatever the sequences' order: with c_s tiles in
+// sequence s, N(j) = sum_s max(0, c_s - j) tiles have x >= j, so the tile of
+// rank r has the largest x with N(x) > r, found by halving, 4 sequences to a lane
+// (about 0.5 us beside the offsets' load). Where the grid has many turns its
+// tiles are ordered so by bands of 2^band_shift levels only, and within a band
+// sequence by sequence: tiles of one sequence that run together read K and V
+// from memory once (255 prompts of up to 2,000 tokens at 32 / 8 heads of 128
+// 4,290 -> 2,750 us; but 16 of 200 at 16 / 4 of 256, one turn, 23.8 -> 25.5).
+//
+// More sequences: sequence s owns the ids from floor(cu[s] G / RW) + s on, as
+// many as it has tiles or one more, and is found among them by steps of 64: one
+// of 5,000 in 3 loads (a prefix sum over all offsets took longer than a short
+// sequence's attention: 2,000 sequences of 64 tokens at 12 / 12 heads of 64 278
+// -> 178 us, 5,000 of 1 to 8 at 32 / 8 of 128 552 -> 304).
 constexpr int LEVEL_SEQS = 256;
-template <int RW, int NW>
+template <int RW>
 __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile, int& c0, int& n, int& x) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lane = threadIdx.x & 63;
     // offsets outside [0, T] are clamped: no row out of range is touched
     auto at = [&](int s) { return max(0, min(p.cu[s], p.T)); };
     auto tiles = [&](int a, int b) { return b > a ? ((b - a) * p.G + RW - 1) / RW : 0; };
@@ -134,9 +145,11 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
             for (int i = 0; i < 4; i++) k += max(0, c[i] - j);
             return wave_sum(k);
         };
-        int lo = 0, hi = wave_max(most) - 1, after = 0;  // N(lo) > tile; after = N(hi + 1)
+        // in bands: N(lo's first level) > tile; after = N(that of hi + 1)
+        const int band = 1 << p.band_shift;
+        int lo = 0, hi = (wave_max(most) - 1) >> p.band_shift, after = 0;
         while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1, k = above(mid);
+            const int mid = (lo + hi + 1) >> 1, k = above(mid << p.band_shift);
             if (k > tile) {
                 lo = mid;
             } else {
@@ -144,68 +157,48 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
                 after = k;
             }
         }
-        // the (tile - N(x + 1))-th sequence that has a tile x
-        int k = 0;
+        // the band's tiles, sequence by sequence, the longest first
+        int d[4], k = 0;
+        lo <<= p.band_shift;
 #pragma unroll
-        for (int i = 0; i < 4; i++) k += c[i] > lo;
+        for (int i = 0; i < 4; i++) {
+            d[i] = max(0, min(c[i] - lo, band));
+            k += d[i];
+        }
         const int incl = wave_prefix(k);
         int r = tile - after - (incl - k), a = 0, b = 0;
         const unsigned long long hit = __ballot(r >= 0 && r < k);
         if (hit == 0) return false;  // offsets that decrease, with counts past 31 bits
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (c[i] > lo && r-- == 0) {
+            if (r >= 0 && r < d[i]) {
                 a = off[i];
                 b = off[i + 1];
+                x = lo + d[i] - 1 - r;
             }
+            r -= d[i];
         }
         const int l = __ffsll((long long)hit) - 1;
         c0 = __builtin_amdgcn_readlane(a, l);
         n = __builtin_amdgcn_readlane(b, l) - c0;
-        x = lo;
+        x = __builtin_amdgcn_readlane(x, l);
         return true;
     }
-    __shared__ int wsum[NW], found[3];
-    const int per = (p.seqs + 64 * NW - 1) / (64 * NW);
-    const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
-    int sum = 0, a = s0 < s1 ? at(s0) : 0;
-    for (int s = s0; s < s1; s++) {
-        const int b = at(s + 1);
-        sum += tiles(a, b);
-        a = b;
+    // The last sequence that starts at or before id `tile`.
+    auto start = [&](int s) { return at(s) * p.G / RW + s; };
+    int s = 0;
+    for (int left = p.seqs; left > 1;) {
+        const int step = (left + 63) / 64, i = lane * step;
+        const int k = __popcll(__ballot(i < left && start(min(s + i, p.seqs)) <= tile));
+        if (k == 0) return false;
+        s += (k - 1) * step;
+        left = min(step, left - (k - 1) * step);
     }
-    const int incl = wave_prefix(sum);
-    if (lane == 63) wsum[wave] = incl;
-    if (tid < 3) found[tid] = 0;
-    __syncthreads();
-    int total = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-        if (w < wave) before += wsum[w];
-        total += wsum[w];
-    }
-    if (tile >= total) return false;
-    const int want = total - 1 - tile;
-    before += incl - sum;
-    if (before <= want && want < before + sum) {
-        int a = at(s0);
-        for (int s = s0; s < s1; s++) {
-            const int b = at(s + 1), k = tiles(a, b);
-            if (want < before + k) {
-                found[0] = a;
-                found[1] = b - a;
-                found[2] = want - before;
-                break;
-            }
-            before += k;
-            a = b;
-        }
-    }
-    __syncthreads();
-    c0 = __builtin_amdgcn_readfirstlane(found[0]);
-    n = __builtin_amdgcn_readfirstlane(found[1]);
-    x = __builtin_amdgcn_readfirstlane(found[2]);
-    return n > 0;  // (0: offsets that decrease, with counts past 31 bits)
+    c0 = at(s);
+    n = at(s + 1) - c0;
+    const int c = tiles(c0, c0 + n);
+    x = c - 1 - (tile - start(s));
+    return x >= 0 && x < c;
 }
 
 // s_waitcnt lgkmcnt(0) that leaves the other counters alone, and keeps memory
@@ -599,7 +592,7 @@ __global__ void __launch_bounds__(64 * RG * KS, OCC) packed_kernel(PackedParams 
     __shared__ int odd[2 * D + 1];
     const int kvh = blockIdx.x % p.Hkv;
     int c0, n, x;
-    if (!find_packed_tile<S::RW, S::NW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
+    if (!find_packed_tile<S::RW>(p, blockIdx.x / p.Hkv, c0, n, x)) return;
     c0 = __builtin_amdgcn_readfirstlane(c0);  // scalars, for the requests' bases
     n = __builtin_amdgcn_readfirstlane(n);
     x = __builtin_amdgcn_readfirstlane(x);

@@ -7,15 +7,18 @@
 
 namespace {
 
-// Tiles of RW rows that the batch can have: each sequence with rows rounds up once.
+// Tiles of RW rows that the batch can have: each sequence with rows rounds up
+// once (many sequences: each has an id, find_packed_tile).
 int64_t tile_bound(const pkv::PackedParams& p, int rw) {
-    return ((int64_t)p.T * p.G + rw - 1) / rw + std::min(p.seqs, p.T);
+    return ((int64_t)p.T * p.G + rw - 1) / rw + (p.seqs > pkv::LEVEL_SEQS ? p.seqs : std::min(p.seqs, p.T));
 }
 
 template <class E, int D, int RG, int KS, int NST, int OCC>
-int launch(const pkv::PackedParams& p, hipStream_t stream) {
+int launch(pkv::PackedParams p, hipStream_t stream) {
     using S = pkv::PackedTile<D, RG, KS, NST>;
     const int64_t grid = tile_bound(p, S::RW) * p.Hkv;
+    // four turns of the grid or more: tiles by bands of 16 levels (find_packed_tile)
+    p.band_shift = grid > (int64_t)4 * OCC * device_cus() ? 4 : 0;
     if (grid * S::THREADS >= (int64_t)1 << 32) return PKV_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((pkv::packed_kernel<E, D, RG, KS, NST, OCC>), dim3((unsigned)grid), dim3(S::THREADS), 0, stream, p);
     return launch_status();

@@ -80,6 +80,34 @@ def check(c, got, what=""):
     assert worst <= 1.0 and not torch.isnan(got[rows]).any()
 
 
+def check_fast(c):
+    """check() for many sequences: those of a length at once."""
+    got, at = run(c), np.cumsum([c["lead"]] + c["lens"])
+    D, G = c["q"].shape[2], c["q"].shape[1] // c["k"].shape[1]
+    u, worst = torch.finfo(c["q"].dtype).eps / 2, 0.0
+    for n in sorted(set(c["lens"]) - {0}):
+        starts = torch.from_numpy(np.flatnonzero(np.array(c["lens"]) == n)).to(got.device)
+        rows = torch.from_numpy(at).to(got.device)[starts][:, None] + torch.arange(n, device=got.device)
+        for part in rows.split(max(1, 20000 // (n * n) + 1)):
+            # [sequences, heads, rows, dims]
+            q, o = (x[part].double().transpose(1, 2) for x in (c["q"], got))
+            k, v = (x[part].double().transpose(1, 2).repeat_interleave(G, 1) for x in (c["k"], c["v"]))
+            kt, seen = k.transpose(2, 3).contiguous(), torch.ones(n, n, dtype=torch.bool, device=got.device).tril()
+            w = torch.softmax(torch.where(seen, q @ kt * c["scale"], -float("inf")), -1)
+            S = torch.where(seen, q.abs() @ kt.abs() * c["scale"], 0).amax(-1, keepdim=True)
+            e = 2 * (D + 16) * 2.0 ** -24 * S + 2.0 ** -20
+            want, A = w @ v, w @ v.abs()
+            m = torch.arange(1, n + 1, device=got.device, dtype=torch.float64)[:, None]
+            tol = (u + e + m * 2.0 ** -24) * A + (2 * u + e) * want.abs()
+            err = ((o - want).abs() / tol).max()
+            assert not torch.isnan(o).any()
+            worst = max(worst, float(err))
+    print(f"{len(c['lens'])} sequences: worst error over bound {worst:.3f}", flush=True)
+    assert worst <= 1.0
+    end = c["lead"] + sum(c["lens"])
+    assert (got[:c["lead"]] == 7).all() and (got[end:] == 7).all()
+
+
 LENS = [[1], [2, 1, 0, 5], [31, 32, 33, 0], [63, 64, 65, 127, 128, 129], [300, 1, 700], [1025]]
 
 
@@ -306,6 +334,15 @@ def test_every_shape_of_workgroup(dev, D, lens, Hq, Hkv):
     """Batches that are shared out among a workgroup's waves by keys, by both and by rows."""
     c = inputs(lens, Hq, Hkv, D, "bf16", D + len(lens), dev, gate=D == 256)
     check(c, run(c), f"D {D} {len(lens)} x {lens[0]} heads {Hq}/{Hkv}")
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv", [
+    ([(37 * i) % 200 for i in range(200)], 32, 8), ([0] * 3 + [260] * 120, 16, 16), ([(53 * i) % 61 for i in range(256)], 64, 16),
+    ([(53 * i) % 9 for i in range(5000)], 4, 2), ([0] * 300 + [700, 0, 1], 8, 2), ([(29 * i) % 97 for i in range(257)], 8, 1)])
+def test_many_turns_and_many_sequences(dev, lens, Hq, Hkv):
+    """Grids of many turns (tiles in bands of levels), and more sequences than a wave holds offsets of, empty ones among
+    them."""
+    check_fast(inputs(lens, Hq, Hkv, 256, "bf16", len(lens), dev, lead=5, tail=3))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
