@@ -36,16 +36,19 @@ int launch(pkv::PackedParams p, hipStream_t stream) {
 // 37, 4,000 44 / 44 / 70. The estimate takes the fastest, or one within 10 %, in
 // all 35 batches that were timed.
 struct Shape {
-    int rows, ks, places;  // rows of a workgroup, key groups, workgroups a CU holds
+    int rows;      // of a workgroup
+    double pace;   // tiles of a row at a time
+    int places;    // workgroups a CU holds
+    double start;  // A
 };
-int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[3], double start) {
+int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[4]) {
     const double tiles = (double)p.T / p.seqs / 32;
     int best = 0;
     double least = 0;
-    for (int i = 0; i < 3; i++) {
+    for (int i = 0; i < 4; i++) {
         const Shape& s = shapes[i];
         const double turns = (double)tile_bound(p, s.rows) * p.Hkv / ((double)s.places * device_cus());
-        const double t = std::max(tiles / s.ks + start, turns * (tiles / (2 * s.ks) + start));
+        const double t = std::max(tiles / s.pace + s.start, turns * (tiles / (2 * s.pace) + s.start));
         if (i == 0 || t < least) best = i, least = t;
     }
     return best;
@@ -54,26 +57,29 @@ int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[3], double star
 template <class E>
 int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
     if (D == 64) {
-        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 4}, {128, 1, 5}};
-        switch (best_shape(p, shapes, 10)) {
+        static constexpr Shape shapes[4] = {{32, 4, 2, 10}, {64, 2, 4, 10}, {128, 1, 5, 10}, {32, 0.5, 16, 13}};
+        switch (best_shape(p, shapes)) {
             case 0: return launch<E, 64, 1, 4, 2, 1>(p, stream);
             case 1: return launch<E, 64, 2, 2, 2, 4>(p, stream);
-            default: return launch<E, 64, 4, 1, 2, 5>(p, stream);
+            case 2: return launch<E, 64, 4, 1, 2, 5>(p, stream);
+            default: return launch<E, 64, 1, 1, 1, 4>(p, stream);
         }
     }
     if (D == 128) {
-        static constexpr Shape shapes[3] = {{32, 4, 2}, {64, 2, 2}, {128, 1, 3}};
-        switch (best_shape(p, shapes, 20)) {
+        static constexpr Shape shapes[4] = {{32, 4, 2, 20}, {64, 2, 2, 20}, {128, 1, 3, 20}, {32, 0.5, 9, 22}};
+        switch (best_shape(p, shapes)) {
             case 0: return launch<E, 128, 1, 4, 1, 2>(p, stream);
             case 1: return launch<E, 128, 2, 2, 2, 2>(p, stream);
-            default: return launch<E, 128, 4, 1, 2, 3>(p, stream);
+            case 2: return launch<E, 128, 4, 1, 2, 3>(p, stream);
+            default: return launch<E, 128, 1, 1, 1, 3>(p, stream);
         }
     }
-    static constexpr Shape shapes[3] = {{32, 4, 1}, {64, 2, 1}, {128, 1, 2}};
-    switch (best_shape(p, shapes, 25)) {
+    static constexpr Shape shapes[4] = {{32, 4, 1, 25}, {64, 2, 1, 25}, {128, 1, 2, 25}, {32, 0.5, 4, 33}};
+    switch (best_shape(p, shapes)) {
         case 0: return launch<E, 256, 1, 4, 1, 1>(p, stream);
         case 1: return launch<E, 256, 2, 2, 2, 1>(p, stream);
-        default: return launch<E, 256, 4, 1, 2, 2>(p, stream);
+        case 2: return launch<E, 256, 4, 1, 2, 2>(p, stream);
+        default: return launch<E, 256, 1, 1, 1, 1>(p, stream);
     }
 }
 
