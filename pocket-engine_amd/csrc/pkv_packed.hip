@@ -24,10 +24,10 @@
 // reads are even, and the softmax between them is what other waves of the SIMD
 // cover. Wider waves (64 rows, half the LDS reads) leave one wave to a SIMD and
 // were slower (16,384 tokens at 32 / 8 heads of 128 2,360 us against 2,010).
-// That prompt runs at 1,100 TFLOP/s (81 % of the 1,361 that a library product of
-// 16,384^3 reaches), its matrix units busy 60 % at 1.7 GHz; 24 prompts of 60 to
-// 4,096 tokens 364 us, 898 TFLOP/s; one of 4,096 at 24 / 4 heads of 256 212 us,
-// 971 TFLOP/s. Batches whose longest prompt alone outlasts the rest are bound by
+// That prompt runs at 1,080 to 1,140 TFLOP/s (80 % of the 1,361 that a library
+// product of 16,384^3 reaches), its matrix units busy 60 % at 1.7 GHz; 24 prompts
+// of 60 to 4,096 tokens 371 us, 881 TFLOP/s; one of 4,096 at 24 / 4 heads of 256
+// 216 us, 955 TFLOP/s (cards differ by 5 %). Batches whose longest prompt alone outlasts the rest are bound by
 // that prompt's chain of tiles (1.1 to 1.3 us each at 256 dims).
 #pragma once
 #include "pkv_rows.h"
