@@ -456,10 +456,11 @@ int pkv_rope_rows(const void* q, int64_t q_row, int64_t q_head, const void* k, i
  * offsets outside [0, T] are clamped. An infinite or NaN value, key or query
  * reaches exactly the rows that attend it. The same call gives the same bits;
  * how a batch's keys are shared out, and with it the last bits of a row, goes
- * by T, seqs and the heads. scale is finite and above 0. PKV_ERR_UNSUPPORTED
- * for other types, dims or groups, T G above 2^30, or sequences times kv heads
- * of 2^24 or more. No workspace. No
- * reference counterpart (the reference attends through its pages only,
+ * by T, seqs and the heads (the mean length T / seqs: many empty sequences, or
+ * rows outside every sequence, make it a slower one). scale is finite and
+ * above 0. PKV_ERR_UNSUPPORTED for other types, dims or groups, T G above 2^30,
+ * or (T G / 128 + seqs) Hkv of 2^24 or more. No workspace. No reference
+ * counterpart (the reference attends through its pages only,
  * src/model.rs:2438-2493). */
 int pkv_attn_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                     const void* v, int64_t v_row, int64_t v_head, const void* gate, int64_t gate_row,
