@@ -78,10 +78,11 @@ int pkv_plan_step(const int32_t* len, const int32_t* held, const int32_t* ntok, 
     p.free_list = free_list, p.free_count = free_count, p.T = T;
     p.pos = pos, p.slot_map = slot_map, p.tok_seq = tok_seq, p.cu = cu, p.limits = limits;
     p.len_out = len_out, p.held_out = held_out, p.free_out = free_count_out, p.status = status;
-    // 256 threads where they hold the rows and, one workgroup, the tokens in two
-    // turns (64 rows 6.9 -> 4.2 us).
+    // 256 threads where they hold the rows and, one workgroup, the tokens and
+    // pages in two turns (64 rows 6.9 -> 4.2 us; but 256 rows with 127,000 tokens in
+    // place 30 -> 15 with 1,024).
     const bool in_place = len_out == len || held_out == held || (free_count_out && free_count_out == free_count);
-    const bool one = in_place && (T <= 2048 || nrows == 0), small = nrows <= 256 && (!one || T <= 512);
+    const bool one = in_place && (T <= 2048 || nrows == 0), small = nrows <= 256 && (!in_place || T <= 512);
     const int threads = small ? 256 : 1024;
     const dim3 grid(in_place ? 1 : std::max(1, std::min(256, (T + threads - 1) / threads)));
     const hipStream_t hs = (hipStream_t)stream;
