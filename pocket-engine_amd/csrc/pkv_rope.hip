@@ -151,10 +151,10 @@ __device__ __forceinline__ float2 turn_of(int pos, float inv) {
 // 8 heads of 128, 336 MB, take 50 us, 6.7 TB/s (a copy of 2 GiB 4.9; part of the
 // rows stays in the last-level cache between calls). A few tokens are bound by
 // the chain position -> angle -> row, 5.5 us for 64.
-constexpr int ROPE_TOKENS = 8;  // tb at most
+constexpr int rope_tokens(int D) { return 2048 / D; }  // tb at most (8 KiB of cos / sin)
 template <class E, int D, bool ADJ, bool STREAM>
 __global__ void __launch_bounds__(256) rope_rows_kernel(RopeParams p, int tb) {
-    __shared__ __align__(16) float cs[ROPE_TOKENS][2][D / 2];  // cos, sin
+    __shared__ __align__(16) float cs[rope_tokens(D)][2][D / 2];  // cos, sin
     constexpr int LPH = D / 16, HPB = 256 / LPH;               // lanes per head, heads at a time
     const int tid = threadIdx.x, t0 = blockIdx.x * tb, u = tid % LPH;
     const int H = p.Hq + p.Hkv, tokens = min(tb, p.T - t0);

@@ -36,7 +36,7 @@ void launch_rope(const pkv::RopeParams& p, hipStream_t stream) {
     // Tokens a workgroup: as many as give its threads two and a half (token,
     // head) pairs each, while that leaves 2,048 workgroups.
     int tb = 1;
-    while (tb < pkv::ROPE_TOKENS && 2 * tb * (p.Hq + p.Hkv) * D <= 10240 && p.T / (2 * tb) >= 2048) tb *= 2;
+    while (tb < pkv::rope_tokens(D) && 2 * tb * (p.Hq + p.Hkv) * D <= 10240 && p.T / (2 * tb) >= 2048) tb *= 2;
     // Stores that leave no lines behind, where the rows pass what the caches keep
     // for their reader: 16,384 rows at 32 / 8 heads of 128 (168 MB) 65 -> 52 us,
     // with the attention over 16 prompts of them 244 -> 246. Below, the reader
