@@ -346,6 +346,25 @@ def test_many_turns_and_many_sequences(dev, lens, Hq, Hkv):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_short_sequences(dev, D, dtype):
+    """Gates, rows outside the sequences, and values that are not finite, where a wave has a tile for itself."""
+    lens = [1 + 7 * i % 9 for i in range(600)]
+    c = inputs(lens, 4, 2, D, dtype, 3 * D, dev, gate=True, lead=2, tail=2)
+    got = run(c)
+    check(c, got, f"D {D} {dtype}")
+    assert (got[:2] == 7).all() and (got[-2:] == 7).all()
+    y = dict(c, v=c["v"].clone())
+    at = 2 + int(np.cumsum(lens)[299]) + 1  # the second row of a sequence of 4
+    assert lens[300] == 4
+    y["v"][at, 0, 3], y["v"][0], y["v"][-1] = float("nan"), float("nan"), float("inf")
+    hit = run(y)
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[at:at + 3, :2, 3] = False
+    assert torch.equal(hit[same], got[same]) and torch.isnan(hit[at:at + 3, :2, 3]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_scores_that_jump(dev, dtype):
     """A key now and then scores far above all before it, in tiles of any key group, for some rows only."""
     for D, n in ((64, 700), (128, 333), (256, 130)):
